@@ -1,0 +1,258 @@
+"""The 8-bit linear path as cases to time and to check: rows are held as e4m3
+codes with one power-of-two scale for each 128 consecutive values (the last
+block of a row may be shorter).
+
+Kinds of case:
+  norm      residual addition and RMS norm, its output in 8 bits; the sum
+            comes back too, as the residual stream of the next layer
+  quantize  rows of F32, BF16 or F16 as codes and scales: a weight at model
+            load, an activation ahead of a linear layer
+  linear    a linear layer on two operands in that form, with bias
+
+Formulas.  A block of values y, a = max |y|: the scale is 2^e with e the
+smallest integer >= -127 for which a <= 448 * 2^e; the codes are y * 2^-e
+rounded to e4m3 (nearest even).
+  norm:    s = x + r rounded to the sum's type; y = s / sqrt(mean(s^2) + eps) * weight
+  linear:  dst[m][n] = sum_k x[m][k] w[n][k] + bias[n], x and w as codes times scales
+
+Where `own` is false everything is computed by elementary torch operations
+in 32 bits; where it is true, by the library, through the descriptors that a
+program makes once and keeps.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DEV = "cuda:0"
+BLOCK = 128
+EPS = 1e-6
+TYPE = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+
+
+def listed():
+    return [
+        # the last norm ahead of a head: one token for each guided branch, latency alone
+        dict(name="norm_2_f32", kind="norm", m=2, k=3584, x="f32", s="f32", residual=True),
+        # a text encoder's block over a prompt of 300 tokens, F32 as the graph has it
+        dict(name="norm_300_f32", kind="norm", m=300, k=3584, x="f32", s="f32", residual=True),
+        # a block's norm over all tokens of a 121-frame clip, guided pair: a BF16 branch onto an F32 stream
+        dict(name="norm_63488_bf16", kind="norm", m=63488, k=4096, x="bf16", s="f32", residual=True),
+        # an odd number of rows of an odd width, no residual
+        dict(name="norm_1237_bf16", kind="norm", m=1237, k=1552, x="bf16", s="bf16", residual=False),
+        # a projection's weight quantised at model load
+        dict(name="quantize_weight_f16", kind="quantize", m=4096, k=4096, x="f16"),
+        # the inner activation of a feed-forward pair
+        dict(name="quantize_16000_bf16", kind="quantize", m=16000, k=16384, x="bf16"),
+        # the time embedding's and the modulations' layers: one row per guided branch
+        dict(name="linear_2", kind="linear", m=2, n=16384, k=4096, out="f32", bias=True),
+        # a text block's projection over the prompt
+        dict(name="linear_300", kind="linear", m=300, n=4096, k=4096, out="f32", bias=True),
+        # odd sizes: tokens and outputs that end inside a tile, a last block of 16 values
+        dict(name="linear_997_odd", kind="linear", m=997, n=1540, k=3600, out="bf16", bias=True),
+        # a visual block's projection at the smallest video
+        dict(name="linear_1280", kind="linear", m=1280, n=4096, k=4096, out="bf16", bias=True),
+        # the same projection at 121 frames, guided pair
+        dict(name="linear_63488", kind="linear", m=63488, n=4096, k=4096, out="f32", bias=True),
+        # the second layer of a feed-forward pair over half such a clip
+        dict(name="linear_16000_ffn", kind="linear", m=15872, n=4096, k=16384, out="bf16", bias=False),
+    ]
+
+
+def log_int(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "quantize", "linear", "linear"])
+    if kind == "linear":
+        if rng.random() < 0.5:
+            n, k = rng.choice([(4096, 4096), (16384, 4096), (4096, 16384), (4096, 1024), (1024, 4096), (1536, 3584), (64, 4096)])
+        else:
+            n, k = 4 * log_int(rng, 1, 4096), 16 * log_int(rng, 1, 1024)
+        m = log_int(rng, 1, min(63488, 63488 * 4096 * 4096 // (n * k)))
+        return dict(kind=kind, m=m, n=n, k=k, out=rng.choice(["f32", "bf16"]), bias=rng.random() < 0.75)
+    k = rng.choice([1024, 1536, 3584, 4096, 16384]) if rng.random() < 0.5 else 16 * log_int(rng, 1, 1024)
+    m = log_int(rng, 1, min(63488, 63488 * 4096 // k))
+    x = rng.choice(["f32", "bf16"])
+    if kind == "quantize":
+        return dict(kind=kind, m=m, k=k, x=rng.choice([x, "f16"]))
+    residual = rng.random() < 0.75
+    return dict(kind=kind, m=m, k=k, x=x, s=rng.choice(["f32", "bf16"]) if residual else x, residual=residual)
+
+
+# ---------------------------------------------------------------------------
+# the plain forms
+# ---------------------------------------------------------------------------
+
+def blocks_of(k):
+    return (k + BLOCK - 1) // BLOCK
+
+
+def padded(y):
+    """(M, K) as (M, blocks, 128), zeros behind the last value."""
+    m, k = y.shape
+    return torch.nn.functional.pad(y, (0, blocks_of(k) * BLOCK - k)).view(m, -1, BLOCK)
+
+
+def quantized(y):
+    """Codes (M, K) and scales (M, blocks) of F32 rows."""
+    b = padded(y)
+    part, power = torch.frexp(b.abs().amax(dim=2))
+    e = torch.clamp(power - 9 + (part > 0.875).to(power.dtype), min=-127)
+    codes = torch.ldexp(b, -e[:, :, None]).view(y.shape[0], -1)[:, :y.shape[1]].to(torch.float8_e4m3fn)
+    return codes.contiguous(), (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def values(codes, scales):
+    """F32 rows of codes and scales."""
+    return codes.float() * scales.float().repeat_interleave(BLOCK, dim=1)[:, :codes.shape[1]]
+
+
+def plain_norm(x, weight, residual, s_type):
+    s = x.float() if residual is None else (x.float() + residual.float()).to(s_type).float()
+    rstd = 1.0 / torch.sqrt(s.square().mean(dim=1, keepdim=True) + EPS)
+    codes, scales = quantized(s * rstd * weight)
+    return {"codes": codes, "scales": scales} if residual is None else {"codes": codes, "scales": scales, "sum": s.to(s_type)}
+
+
+def plain_linear(x, w, bias, out):
+    y = values(*x) @ values(*w).t()
+    return (y if bias is None else y + bias).to(out)
+
+
+# ---------------------------------------------------------------------------
+# the cases
+# ---------------------------------------------------------------------------
+
+def rows(gen, m, k, dtype=torch.float32, scale=1.0):
+    """Normal values, a hundredth of the columns eight times as large."""
+    col = torch.where(torch.rand(k, generator=gen, device=DEV) < 0.01, 8.0 * scale, scale)
+    return torch.randn((m, k), generator=gen, device=DEV).mul_(col).to(dtype)
+
+
+def eight_bit(gen, m, k, scale):
+    """Random rows as codes and scales, the scales' rows padded to whole words as the library asks."""
+    codes, scales = quantized(rows(gen, m, k, scale=scale))
+    store = torch.zeros((m, (scales.shape[1] + 3) // 4 * 4), dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    store[:, :scales.shape[1]].copy_(scales)
+    return codes, store[:, :scales.shape[1]]
+
+
+def library():
+    path = os.path.join(os.getcwd(), "kandinsky.cpp_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import kd_f8
+    return kd_f8
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    m, k = case["m"], case["k"]
+    st = {"kind": case["kind"]}
+    if case["kind"] == "linear":
+        n = case["n"]
+        st["x"], st["w"] = eight_bit(gen, m, k, 1.0), eight_bit(gen, n, k, k ** -0.5)
+        st["bias"] = torch.randn(n, generator=gen, device=DEV) * 0.1 if case["bias"] else None
+        st["type"] = TYPE[case["out"]]
+        if own:
+            f8 = library()
+            st["out"] = torch.empty((m, n), dtype=st["type"], device=DEV)
+            st["desc"] = f8.linear_desc(f8.Rows(*st["x"]), f8.Rows(*st["w"]), st["out"], bias=st["bias"])
+        return st
+    st["x"] = rows(gen, m, k, TYPE[case["x"]], 0.02 if case["x"] == "f16" else 1.0)
+    if case["kind"] == "norm":
+        st["weight"] = 1.0 + 0.2 * torch.randn(k, generator=gen, device=DEV)
+        st["type"] = TYPE[case["s"]]
+        st["residual"] = rows(gen, m, k, st["type"], 4.0) if case["residual"] else None
+    if own:
+        f8 = library()
+        q = f8.empty_rows((m,), k, DEV)
+        st["out"] = {"codes": q.codes, "scales": q.scales}
+        if case["kind"] == "quantize":
+            st["desc"] = f8.quantize_desc(st["x"], q)
+        else:
+            s = torch.empty((m, k), dtype=st["type"], device=DEV) if case["residual"] else None
+            if s is not None:
+                st["out"]["sum"] = s
+            st["desc"] = f8.norm_desc(st["x"], st["weight"], q, residual=st["residual"], sum=s, eps=EPS)
+    return st
+
+
+def run(state):
+    if own:
+        library().run(state["desc"])
+        return state["out"]
+    if state["kind"] == "linear":
+        return plain_linear(state["x"], state["w"], state["bias"], state["type"])
+    if state["kind"] == "norm":
+        return plain_norm(state["x"], state["weight"], state["residual"], state["type"])
+    codes, scales = quantized(state["x"].float())
+    return {"codes": codes, "scales": scales}
+
+
+def work(case):
+    m, k = case["m"], case["k"]
+    row = k + blocks_of(k)
+    if case["kind"] == "linear":
+        n = case["n"]
+        return {"bytes": (m + n) * row + m * n * SIZE[case["out"]] + (4 * n if case["bias"] else 0), "flops": 2 * m * n * k}
+    if case["kind"] == "quantize":
+        return {"bytes": m * (k * SIZE[case["x"]] + row), "flops": 2 * m * k}
+    s = 2 * SIZE[case["s"]] if case["residual"] else 0
+    return {"bytes": m * (k * (SIZE[case["x"]] + s) + row) + 4 * k, "flops": 7 * m * k}
+
+
+# ---------------------------------------------------------------------------
+# the definition in 64 bits
+# ---------------------------------------------------------------------------
+
+def exact_e4m3(v):
+    """The nearest e4m3 value of each |v| <= 448, ties to the even one: 2^-9 apart below 2^-6, then 8 to a binade."""
+    _, e = torch.frexp(v)
+    step = torch.exp2((e.double() - 4).clamp(min=-9.0))
+    return torch.round(v / step) * step
+
+
+def exact_rows(y):
+    m, k = y.shape
+    b = blocks_of(k)
+    full = torch.zeros((m, b * BLOCK), dtype=torch.float64, device=y.device)
+    full[:, :k] = y
+    full = full.view(m, b, BLOCK)
+    top = full.abs().amax(dim=2)
+    # log2 gives the exponent to within one; the inequality itself decides
+    e = torch.ceil(torch.log2(torch.where(top > 0, top, 1.0) / 448.0)) - 1
+    for _ in range(2):
+        e = torch.where(top > 448.0 * torch.exp2(e), e + 1, e)
+    scale = torch.exp2(torch.where(top > 0, e, -127.0).clamp(min=-127.0))
+    return {"codes": exact_e4m3(full / scale[:, :, None]).view(m, -1)[:, :k], "scales": scale}
+
+
+def exact_values(codes, scales):
+    v = codes.to(torch.float64)
+    for j in range(scales.shape[1]):
+        v[:, j * BLOCK:(j + 1) * BLOCK] *= scales[:, j:j + 1].to(torch.float64)
+    return v
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    if case["kind"] == "linear":
+        y = torch.mm(exact_values(*st["x"]), exact_values(*st["w"]).t())
+        return y if st["bias"] is None else y.add_(st["bias"].double())
+    x = st["x"].double()
+    if case["kind"] == "quantize":
+        return exact_rows(x)
+    if st["residual"] is None:
+        s, total = x, {}
+    else:
+        total = {"sum": x + st["residual"].double()}
+        s = total["sum"].to(st["type"]).double()
+    y = s / torch.sqrt((s * s).sum(dim=1, keepdim=True) / case["k"] + EPS) * st["weight"].double()
+    return {**exact_rows(y), **total}

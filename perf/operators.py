@@ -7,7 +7,8 @@ Kinds of case:
             comes back too, as the residual stream of the next layer
   quantize  rows of F32, BF16 or F16 as codes and scales: a weight at model
             load, an activation ahead of a linear layer
-  linear    a linear layer on two operands in that form, with bias
+  linear    a linear layer on two operands in that form, with bias; its
+            output in BF16
 
 Formulas.  A block of values y, a = max |y|: the scale is 2^e with e the
 smallest integer >= -127 for which a <= 448 * 2^e; the codes are y * 2^-e
@@ -49,17 +50,17 @@ def listed():
         # the inner activation of a feed-forward pair
         dict(name="quantize_16000_bf16", kind="quantize", m=16000, k=16384, x="bf16"),
         # the time embedding's and the modulations' layers: one row per guided branch
-        dict(name="linear_2", kind="linear", m=2, n=16384, k=4096, out="f32", bias=True),
+        dict(name="linear_2", kind="linear", m=2, n=16384, k=4096, bias=True),
         # a text block's projection over the prompt
-        dict(name="linear_300", kind="linear", m=300, n=4096, k=4096, out="f32", bias=True),
+        dict(name="linear_300", kind="linear", m=300, n=4096, k=4096, bias=True),
         # odd sizes: tokens and outputs that end inside a tile, a last block of 16 values
-        dict(name="linear_997_odd", kind="linear", m=997, n=1540, k=3600, out="bf16", bias=True),
+        dict(name="linear_997_odd", kind="linear", m=997, n=1540, k=3600, bias=True),
         # a visual block's projection at the smallest video
-        dict(name="linear_1280", kind="linear", m=1280, n=4096, k=4096, out="bf16", bias=True),
+        dict(name="linear_1280", kind="linear", m=1280, n=4096, k=4096, bias=True),
         # the same projection at 121 frames, guided pair
-        dict(name="linear_63488", kind="linear", m=63488, n=4096, k=4096, out="f32", bias=True),
+        dict(name="linear_63488", kind="linear", m=63488, n=4096, k=4096, bias=True),
         # the second layer of a feed-forward pair over half such a clip
-        dict(name="linear_16000_ffn", kind="linear", m=15872, n=4096, k=16384, out="bf16", bias=False),
+        dict(name="linear_16000_ffn", kind="linear", m=15872, n=4096, k=16384, bias=False),
     ]
 
 
@@ -75,7 +76,7 @@ def draw(rng):
         else:
             n, k = 4 * log_int(rng, 1, 4096), 16 * log_int(rng, 1, 1024)
         m = log_int(rng, 1, min(63488, 63488 * 4096 * 4096 // (n * k)))
-        return dict(kind=kind, m=m, n=n, k=k, out=rng.choice(["f32", "bf16"]), bias=rng.random() < 0.75)
+        return dict(kind=kind, m=m, n=n, k=k, bias=rng.random() < 0.75)
     k = rng.choice([1024, 1536, 3584, 4096, 16384]) if rng.random() < 0.5 else 16 * log_int(rng, 1, 1024)
     m = log_int(rng, 1, min(63488, 63488 * 4096 // k))
     x = rng.choice(["f32", "bf16"])
@@ -120,9 +121,9 @@ def plain_norm(x, weight, residual, s_type):
     return {"codes": codes, "scales": scales} if residual is None else {"codes": codes, "scales": scales, "sum": s.to(s_type)}
 
 
-def plain_linear(x, w, bias, out):
+def plain_linear(x, w, bias):
     y = values(*x) @ values(*w).t()
-    return (y if bias is None else y + bias).to(out)
+    return (y if bias is None else y + bias).to(torch.bfloat16)
 
 
 # ---------------------------------------------------------------------------
@@ -159,10 +160,9 @@ def prepare(case, seed):
         n = case["n"]
         st["x"], st["w"] = eight_bit(gen, m, k, 1.0), eight_bit(gen, n, k, k ** -0.5)
         st["bias"] = torch.randn(n, generator=gen, device=DEV) * 0.1 if case["bias"] else None
-        st["type"] = TYPE[case["out"]]
         if own:
             f8 = library()
-            st["out"] = torch.empty((m, n), dtype=st["type"], device=DEV)
+            st["out"] = torch.empty((m, n), dtype=torch.bfloat16, device=DEV)
             st["desc"] = f8.linear_desc(f8.Rows(*st["x"]), f8.Rows(*st["w"]), st["out"], bias=st["bias"])
         return st
     st["x"] = rows(gen, m, k, TYPE[case["x"]], 0.02 if case["x"] == "f16" else 1.0)
@@ -189,7 +189,7 @@ def run(state):
         library().run(state["desc"])
         return state["out"]
     if state["kind"] == "linear":
-        return plain_linear(state["x"], state["w"], state["bias"], state["type"])
+        return plain_linear(state["x"], state["w"], state["bias"])
     if state["kind"] == "norm":
         return plain_norm(state["x"], state["weight"], state["residual"], state["type"])
     codes, scales = quantized(state["x"].float())
@@ -201,7 +201,7 @@ def work(case):
     row = k + blocks_of(k)
     if case["kind"] == "linear":
         n = case["n"]
-        return {"bytes": (m + n) * row + m * n * SIZE[case["out"]] + (4 * n if case["bias"] else 0), "flops": 2 * m * n * k}
+        return {"bytes": (m + n) * row + 2 * m * n + (4 * n if case["bias"] else 0), "flops": 2 * m * n * k}
     if case["kind"] == "quantize":
         return {"bytes": m * (k * SIZE[case["x"]] + row), "flops": 2 * m * k}
     s = 2 * SIZE[case["s"]] if case["residual"] else 0

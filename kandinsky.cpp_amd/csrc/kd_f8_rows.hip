@@ -1,0 +1,278 @@
+// kd_f8_rows.hip - rows into 8 bits (include/kd_f8.h): e4m3 codes with one
+// E8M0 scale for each block of 128 values.
+//
+//   quantize_kernel  rows of F32, BF16 or F16
+//   norm_kernel      residual addition and RMS norm (RMSNorm,
+//                    src/core/module.hpp:163-180), its output in 8 bits
+//
+// In both a thread holds 8 consecutive values, so that the 16 lanes of a
+// DPP row hold one block: its largest magnitude takes four DPP steps, and
+// the scale and the codes follow without LDS.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/kd_f8.h"
+#include "kd_f8_kernel.h"
+#include "kd_fa_device.h"
+
+namespace kdfa {
+
+// Eight values as loaded, and as F32.
+template <int TYPE> struct F8Src;
+template <> struct F8Src<KD_F8_TYPE_F32> {
+    f32x4 u, v;
+    __device__ __forceinline__ void load(const char *row, int col) {
+        u = *reinterpret_cast<const f32x4 *>(row + (int64_t)col * 4);
+        v = *reinterpret_cast<const f32x4 *>(row + (int64_t)col * 4 + 16);
+    }
+    __device__ __forceinline__ void get(float y[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { y[e] = u[e]; y[4 + e] = v[e]; }
+    }
+    // F32 rounds to itself
+    static __device__ __forceinline__ void round_store(char *row, int col, float y[8], bool in) {
+        if (in) {
+            *reinterpret_cast<f32x4 *>(row + (int64_t)col * 4) = (f32x4){y[0], y[1], y[2], y[3]};
+            *reinterpret_cast<f32x4 *>(row + (int64_t)col * 4 + 16) = (f32x4){y[4], y[5], y[6], y[7]};
+        }
+    }
+};
+template <> struct F8Src<KD_F8_TYPE_BF16> {
+    u32x4 w;
+    __device__ __forceinline__ void load(const char *row, int col) { w = ld16(row + (int64_t)col * 2); }
+    __device__ __forceinline__ void get(float y[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { y[2 * e] = bf16_lo(w[e]); y[2 * e + 1] = bf16_hi(w[e]); }
+    }
+    static __device__ __forceinline__ void round_store(char *row, int col, float y[8], bool in) {
+        u32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            o[e] = Elem<__bf16>::pack2(y[2 * e], y[2 * e + 1]);
+            y[2 * e] = bf16_lo(o[e]);
+            y[2 * e + 1] = bf16_hi(o[e]);
+        }
+        if (in) *reinterpret_cast<u32x4 *>(row + (int64_t)col * 2) = o;
+    }
+};
+template <> struct F8Src<KD_F8_TYPE_F16> {
+    u32x4 w;
+    __device__ __forceinline__ void load(const char *row, int col) { w = ld16(row + (int64_t)col * 2); }
+    __device__ __forceinline__ void get(float y[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { y[2 * e] = f16_lo(w[e]); y[2 * e + 1] = f16_hi(w[e]); }
+    }
+};
+
+// the larger of x and x of the lane that DPP control CTRL names
+template <int CTRL>
+static __device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+    return x > o ? x : o;
+}
+
+// Eight values of a block (its 16 lanes call together) as codes; the block's
+// scale byte.  Magnitudes are compared as bits, where NaN is above infinity
+// and infinity above every number.  max|y| = f * 2^E with 1 <= f < 2: 2^e is
+// 2^(E - 8) for f <= 1.75 (448 = 1.75 * 2^8), else 2^(E - 7): adding
+// 0x1fffff to the bits carries into the exponent for f > 1.75 alone.  A
+// magnitude with an exponent field below 8 takes byte 0, so does zero.  2^-e
+// is a normal number for every byte up to 247, the largest number's, and the
+// product by it is exact (what underflows is far below half a code), so that
+// the conversion's is the only rounding.
+static __device__ __forceinline__ u32x2 to_f8(const float y[8], uint32_t &byte) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
+        m = b > m ? b : m;
+    }
+    m = max_dpp<0xb1>(m);    // lane ^ 1
+    m = max_dpp<0x4e>(m);    // lane ^ 2
+    m = max_dpp<0x141>(m);   // 7 - lane of each 8
+    m = max_dpp<0x140>(m);   // 15 - lane
+    const uint32_t f = (m + 0x1fffffu) >> 23;
+    const bool bad = m >= 0x7f800000u;
+    byte = bad ? 255u : (f > 8 ? f - 8 : 0);
+    const float inv = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((254u - byte) << 23);
+    u32x2 c;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        int w = 0;
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h] * inv, y[4 * h + 1] * inv, w, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2] * inv, y[4 * h + 3] * inv, w, true);
+        c[h] = (uint32_t)w;
+    }
+    return c;
+}
+
+// ---------------------------------------------------------------------------
+// quantize_kernel: bound by HBM.  16 lanes take a block; the blocks of all
+// rows are counted through, 64 to a workgroup, four of them (64 bytes of
+// 16-bit x a lane) loaded before the first is stored.
+// ---------------------------------------------------------------------------
+template <int TYPE>
+__global__ __launch_bounds__(256) void quantize_kernel(F8RowsArgs a) {
+    constexpr int kU = kF8QuantBlocks / 16;
+    const int lane16 = threadIdx.x & 15;
+    const int team = threadIdx.x >> 4;
+    const float rcp = 1.0f / (float)a.blocks;
+    const int64_t total = (int64_t)a.M * a.blocks;
+    for (int64_t t0 = (int64_t)blockIdx.x * kF8QuantBlocks; t0 < total; t0 += (int64_t)gridDim.x * kF8QuantBlocks) {
+        const int64_t row0 = (int64_t)((uint64_t)t0 / (uint32_t)a.blocks);
+        const int rem0 = (int)(t0 - row0 * a.blocks);
+        F8Src<TYPE> s[kU];
+        int64_t row[kU];
+        int col[kU], blk[kU];
+        bool in[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int i = 16 * u + team;
+            // past the end, the last block again (not stored)
+            const int j = t0 + i < total ? i : (int)(total - 1 - t0);
+            const int r = div_small(rem0 + j, a.blocks, rcp);
+            row[u] = row0 + r;
+            blk[u] = rem0 + j - r * a.blocks;
+            col[u] = blk[u] * kF8Block + 8 * lane16;
+            in[u] = col[u] < a.K;
+            s[u].load(a.x + row[u] * a.x_nb1, in[u] ? col[u] : 0);
+            in[u] = in[u] && t0 + i < total;
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            float y[8];
+            s[u].get(y);
+            if (col[u] >= a.K) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+            }
+            uint32_t byte;
+            const u32x2 c = to_f8(y, byte);
+            if (in[u]) {
+                *reinterpret_cast<u32x2 *>(a.codes + row[u] * a.c_nb1 + col[u]) = c;
+                if (lane16 == 0) a.scales[row[u] * a.e_nb1 + blk[u]] = (char)byte;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// norm_kernel: T threads to a row, C chunks of 8 values each, the whole row
+// in registers between its one reading and its writing.  Bound by HBM for
+// many rows, by one row's latency for few.
+// ---------------------------------------------------------------------------
+template <int XT, int ST, bool RES, int T, int C>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
+    constexpr int kRows = T < 256 ? 256 / T : 1;   // rows at once in a workgroup
+    constexpr int kWaves = T / 64;
+    __shared__ float part[2][kWaves];
+    const int tid = threadIdx.x % T;
+    const int lane = threadIdx.x & 63;
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T; row < a.M; row += (int64_t)gridDim.x * kRows) {
+        F8Src<XT> x[C];
+        F8Src<ST> r[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = 8 * (tid + T * c);
+            x[c].load(a.x + row * a.x_nb1, col < a.K ? col : 0);
+            if constexpr (RES) r[c].load(a.residual + row * a.r_nb1, col < a.K ? col : 0);
+        }
+        float y[C][8];
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = 8 * (tid + T * c);
+            const bool in = col < a.K;
+            x[c].get(y[c]);
+            if constexpr (RES) {
+                float z[8];
+                r[c].get(z);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[c][e] += z[e];
+                F8Src<ST>::round_store(a.sum + row * a.s_nb1, col, y[c], in);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[c][e] = in ? y[c][e] : 0.0f;
+                ss += y[c][e] * y[c][e];
+            }
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) ss += __shfl_xor(ss, m, 64);
+        if constexpr (kWaves > 1) {
+            // two buffers in turn: a row's partial sums are read before the
+            // next row's barrier, the row after that writes over them behind it
+            if (lane == 0) part[turn][tid >> 6] = ss;
+            __syncthreads();
+            ss = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) ss += part[turn][w];
+            turn ^= 1;
+        }
+        const float rstd = 1.0f / sqrt_rn(ss / (float)a.K + a.eps);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = 8 * (tid + T * c);
+            const bool in = col < a.K;
+            const f32x4 w0 = *reinterpret_cast<const f32x4 *>(a.weight + (in ? col : 0));
+            const f32x4 w1 = *reinterpret_cast<const f32x4 *>(a.weight + (in ? col : 0) + 4);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = (y[c][e] * rstd) * (e < 4 ? w0[e] : w1[e - 4]);
+                v[e] = in ? p : 0.0f;
+            }
+            uint32_t byte;
+            const u32x2 q = to_f8(v, byte);
+            if (in) {
+                *reinterpret_cast<u32x2 *>(a.codes + row * a.c_nb1 + col) = q;
+                if ((tid & 15) == 0) a.scales[row * a.e_nb1 + (col >> 7)] = (char)byte;
+            }
+        }
+    }
+}
+
+hipError_t launch_f8_quantize(const F8RowsArgs &a, hipStream_t s) {
+    const int64_t want = ((int64_t)a.M * a.blocks + kF8QuantBlocks - 1) / kF8QuantBlocks;
+    const dim3 grid((unsigned)(want < (1 << 22) ? want : 1 << 22));
+    if (a.x_type == KD_F8_TYPE_F32)
+        hipLaunchKernelGGL((quantize_kernel<KD_F8_TYPE_F32>), grid, dim3(256), 0, s, a);
+    else if (a.x_type == KD_F8_TYPE_BF16)
+        hipLaunchKernelGGL((quantize_kernel<KD_F8_TYPE_BF16>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((quantize_kernel<KD_F8_TYPE_F16>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int XT, int ST, bool RES, int T, int C>
+static void launch_norm_tc(const F8RowsArgs &a, hipStream_t s) {
+    constexpr int kRows = T < 256 ? 256 / T : 1;
+    const int64_t want = ((int64_t)a.M + kRows - 1) / kRows;
+    const dim3 grid((unsigned)(want < (1 << 20) ? want : 1 << 20));
+    hipLaunchKernelGGL((norm_kernel<XT, ST, RES, T, C>), grid, dim3(T < 256 ? 256 : T), 0, s, a);
+}
+
+template <int XT, int ST, bool RES>
+static void launch_norm_t(const F8RowsArgs &a, hipStream_t s) {
+    const bool few = a.M <= 1024;
+    if (a.K <= 512) launch_norm_tc<XT, ST, RES, 64, 1>(a, s);
+    else if (a.K <= 2048) few ? launch_norm_tc<XT, ST, RES, 256, 1>(a, s) : launch_norm_tc<XT, ST, RES, 64, 4>(a, s);
+    else if (a.K <= 4096) few ? launch_norm_tc<XT, ST, RES, 256, 2>(a, s) : launch_norm_tc<XT, ST, RES, 64, 8>(a, s);
+    else if (a.K <= 16384) launch_norm_tc<XT, ST, RES, 256, 8>(a, s);
+    else launch_norm_tc<XT, ST, RES, 1024, 8>(a, s);
+}
+
+hipError_t launch_f8_norm(const F8RowsArgs &a, hipStream_t s) {
+    const bool f32 = a.x_type == KD_F8_TYPE_F32;
+    constexpr int F = KD_F8_TYPE_F32, B = KD_F8_TYPE_BF16;
+    if (!a.residual)
+        f32 ? launch_norm_t<F, F, false>(a, s) : launch_norm_t<B, B, false>(a, s);
+    else if (a.s_type == F)
+        f32 ? launch_norm_t<F, F, true>(a, s) : launch_norm_t<B, F, true>(a, s);
+    else
+        f32 ? launch_norm_t<F, B, true>(a, s) : launch_norm_t<B, B, true>(a, s);
+    return hipGetLastError();
+}
+
+}  // namespace kdfa

@@ -236,8 +236,9 @@ def type_id(dtype) -> int:
     raise ValueError(f"no ggml type for {dtype}")
 
 
-def view(t) -> KdFaTensor:
-    """ggml view of a torch tensor of rank <= 4 (shape = ne reversed)."""
+def view(t, type=None) -> KdFaTensor:
+    """ggml view of a torch tensor of rank <= 4 (shape = ne reversed).
+    ``type``: the type id, where it is not the dtype's own."""
     if t is None:
         return KdFaTensor()
     if t.dim() > 4:
@@ -249,7 +250,7 @@ def view(t) -> KdFaTensor:
         shape.append(1)
         strides.append(strides[-1] * shape[-2] if strides else es)
     d = KdFaTensor()
-    d.type = type_id(t.dtype)
+    d.type = type_id(t.dtype) if type is None else type
     for i in range(4):
         d.ne[i] = int(shape[i])
         d.nb[i] = int(strides[i])

@@ -204,6 +204,268 @@ __global__ __launch_bounds__(256) void f8_mm_stream(F8MmArgs a) {
     }
 }
 
+// ---------------------------------------------------------------------------
+// f8_mm_tile: 256 outputs x 256 tokens per workgroup, 4 waves (one per SIMD,
+// 512 registers each), wave w the 128 x 128 quarter (w & 1, w >> 1) as 8 x 8
+// accumulator blocks (256 AGPRs).
+//
+// K advances 128 per stage, whole 128-byte lines of W's and X's rows, which
+// come by DMA into two buffers of W and three of X (32 KB each: all of LDS).
+// In LDS 16-byte chunk c of row r lies at c ^ ((r >> 1) & 7), which spreads
+// the 16 rows of a fragment read over the 64 banks.
+//
+// Step kt goes through W's eight fragments: 8 products of each with the X
+// fragments, which are in registers since the step before.  Meanwhile W's
+// fragments are read two ahead of their products and stage kt + 1's X
+// fragments into the other set, so that LDS is read evenly (32 reads over 64
+// products).  The one barrier stands behind the last of those reads, three
+// quarters of the step through: it frees W's buffer of stage kt and X's of
+// stage kt + 1 for stages kt + 2 and kt + 4, and publishes W of stage kt + 1
+// and X of stage kt + 2.  X, which is another for every workgroup of a
+// column, so has almost two steps for its way; W, whose lines the XCD's other
+// workgroups ask for too, one.
+//
+// A row's scales come as words of four stages, loaded by the lanes that hold
+// the row, a step ahead of their first use.
+// Rows past M or N are the last row again (not stored).  The last steps bring
+// nothing past K: a stage that is not there is the tile's first chunk for
+// every lane, a chunk past K its row's first of that stage, and X's are
+// zeroed in their registers.
+// ---------------------------------------------------------------------------
+constexpr int kTileBuf = 32768;   // 256 rows x 128 k
+
+template <int SEL>
+static __device__ __forceinline__ void mfma_f8_asm(f32x4 &c, const i32x8 &a, const i32x8 &b, uint32_t sa, uint32_t sb) {
+    if constexpr (SEL == 0)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    else if constexpr (SEL == 1)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    else if constexpr (SEL == 2)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb));
+}
+
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void f8_mm_tile(F8MmArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[5 * kTileBuf];
+    lds_t *const sbase = LDS_PTR(char, lds);
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15;
+    const int q4 = lane >> 4;
+    const int wn = wave & 1, wm = wave >> 1;
+    int nt, mt;
+    f8_tile(a, nt, mt);
+    const int n0 = nt * 256, m0 = mt * 256;
+    const int nk = (int)(((uint32_t)a.K + 127) >> 7);   // stages
+    const int whole = a.K >> 7;                         // those of 128 k
+    const int ng = (nk + 3) >> 2;                       // words of scales
+
+    // DMA j of a wave: rows 8 (wave + 4 j) .. +7, lane l the chunk that lies
+    // at l % 8 of row l / 8
+    uint32_t w_off[8], x_off[8];
+    const int dc = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int r = 8 * (wave + 4 * j) + (lane >> 3);
+        w_off[j] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.w_nb1 + (uint32_t)(dc << 4);
+        x_off[j] = (uint32_t)min(r, a.M - 1 - m0) * (uint32_t)a.x_nb1 + (uint32_t)(dc << 4);
+    }
+    const char *const wtile = a.w + (int64_t)n0 * a.w_nb1;
+    const char *const xtile = a.x + (int64_t)m0 * a.x_nb1;
+    auto dma = [&](const char *tile, uint32_t off, int kt, lds_t *buf, int j, auto end_c) __attribute__((always_inline)) {
+        int64_t k0 = (int64_t)kt * 128;
+        if constexpr (decltype(end_c)::value) {
+            off = kt >= nk ? 0 : kt * 128 + 16 * dc < a.K ? off : off - (uint32_t)(dc << 4);
+            k0 = kt >= nk ? 0 : k0;
+        }
+        dma16(tile + k0, off, buf + (wave + 4 * j) * 1024);
+    };
+    auto dma_w = [&](int kt, int buf, int j, auto end_c) __attribute__((always_inline)) {
+        dma(wtile, w_off[j], kt, sbase + buf * kTileBuf, j, end_c);
+    };
+    auto dma_x = [&](int kt, int buf, int j, auto end_c) __attribute__((always_inline)) {
+        dma(xtile, x_off[j], kt, sbase + (2 + buf) * kTileBuf, j, end_c);
+    };
+
+    // scales: row 16 i + l16 of this wave's half
+    uint32_t sw[8], sx[8], nw[8], nx[8];
+    auto load_scales = [&](int g) __attribute__((always_inline)) {
+        const int o = 4 * min(g, ng - 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t rn = (uint32_t)min(128 * wn + 16 * i + l16, a.N - 1 - n0) * (uint32_t)a.ws_nb1;
+            const uint32_t rm = (uint32_t)min(128 * wm + 16 * i + l16, a.M - 1 - m0) * (uint32_t)a.xs_nb1;
+            nw[i] = *reinterpret_cast<const uint32_t *>(a.ws + (int64_t)n0 * a.ws_nb1 + (uint64_t)(rn + o));
+            nx[i] = *reinterpret_cast<const uint32_t *>(a.xs + (int64_t)m0 * a.xs_nb1 + (uint64_t)(rm + o));
+        }
+    };
+
+    // fragments
+    typedef const __attribute__((address_space(3))) u32x4 lds_u4;
+    const uint32_t f_rd = (uint32_t)(l16 * 128 + ((q4 ^ ((l16 >> 1) & 7)) << 4));
+    const uint32_t w_rd = f_rd + 128 * 128 * wn, x_rd = f_rd + 128 * 128 * wm + 2 * kTileBuf;
+    u32x4 fw[4][2], fx[2][8][2];
+    auto read_w = [&](int buf, int i, int h) __attribute__((always_inline)) {
+        fw[i & 3][h] = *reinterpret_cast<lds_u4 *>(sbase + buf * kTileBuf + (w_rd ^ (h << 6)) + i * 2048);
+    };
+    auto read_x = [&](int buf, auto set_c, int j, int h) __attribute__((always_inline)) {
+        fx[decltype(set_c)::value][j][h] = *reinterpret_cast<lds_u4 *>(sbase + buf * kTileBuf + (x_rd ^ (h << 6)) + j * 2048);
+    };
+
+    f32x4 acc[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = (f32x4){};
+
+    int xb = 1;   // the X buffer of stage kt + 1
+    // step kt: byte SEL of the scales' words, W buffer and X set SEL & 1
+    auto step = [&](int kt, auto sel_c, auto end_c) __attribute__((always_inline)) {
+        constexpr int S = decltype(sel_c)::value, P = S & 1;
+        constexpr bool END = decltype(end_c)::value;
+        const int xprev = xb == 0 ? 2 : xb - 1;   // freed by the last step's barrier
+        if constexpr (END) {
+            if (kt >= whole) {
+                // the one stage that ends inside: what lies past K is zero
+                const int left = a.K - kt * 128 - 16 * q4;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    fx[P][j][0] = left > 0 ? fx[P][j][0] : (u32x4){};
+                    fx[P][j][1] = left > 64 ? fx[P][j][1] : (u32x4){};
+                }
+                asm volatile("s_nop 4" ::: "memory");   // (the products are asm: VALU results before they read them)
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int p = 0; p < 64; ++p) {
+            const int i = p >> 3, j = p & 7;
+            if (p == 48) {
+                if constexpr (S == 3) {
+                    // the next words of scales, loaded a step ago (the
+                    // compiler waits for them here)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) asm volatile("" : "+v"(nw[q]), "+v"(nx[q]));
+                }
+                // all but the 8 DMAs of X of stage kt + 3 have landed
+                asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+                __syncthreads();
+                if constexpr (S == 2) load_scales((kt >> 2) + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            mfma_f8_asm<S>(acc[i][j], join(fw[i & 3][0], fw[i & 3][1]), join(fx[P][j][0], fx[P][j][1]), sw[i], sx[j]);
+            __builtin_amdgcn_sched_barrier(0);
+            // X of stage kt + 3, into the buffer that the last step freed
+            if (p < 32 && p % 4 == 0) dma_x(kt + 3, xprev, p / 4, end_c);
+            // W's fragment two on
+            if (i < 6 && (j == 1 || j == 3)) read_w(P, i + 2, j >> 1);
+            // X of stage kt + 1
+            if (i < 4 && (j == 2 || j == 4 || j == 5 || j == 7)) {
+                const int q = 4 * i + (j == 2 ? 0 : j == 4 ? 1 : j == 5 ? 2 : 3);
+                read_x(xb, IC<1 - P>(), q >> 1, q & 1);
+            }
+            if (p >= 48) {
+                if (j % 2 == 0) dma_w(kt + 2, P, (p - 48) / 2, end_c);
+                if (j == 1 || j == 3) read_w(1 - P, i - 6, j >> 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        xb = xb == 2 ? 0 : xb + 1;
+        if constexpr (S == 3) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) { sw[q] = nw[q]; sx[q] = nx[q]; }
+            asm volatile("s_nop 4" ::: "memory");
+        }
+    };
+
+    load_scales(0);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) { sw[q] = nw[q]; sx[q] = nx[q]; }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) asm volatile("" : "+v"(sw[q]), "+v"(sx[q]));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dma_x(0, 0, j, BC<true>());
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dma_w(0, 0, j, BC<true>());
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dma_x(1, 1, j, BC<true>());
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dma_w(1, 1, j, BC<true>());
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dma_x(2, 2, j, BC<true>());
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) read_x(0, IC<0>(), j, h);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) read_w(0, i, h);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+
+    int kt = 0;
+    for (; kt + 7 <= whole; kt += 4) {   // the last step's X is stage kt + 6
+        step(kt, IC<0>(), BC<false>());
+        step(kt + 1, IC<1>(), BC<false>());
+        step(kt + 2, IC<2>(), BC<false>());
+        step(kt + 3, IC<3>(), BC<false>());
+    }
+    for (; kt < nk; kt += 4) {
+        step(kt, IC<0>(), BC<true>());
+        if (kt + 1 < nk) step(kt + 1, IC<1>(), BC<true>());
+        if (kt + 2 < nk) step(kt + 2, IC<2>(), BC<true>());
+        if (kt + 3 < nk) step(kt + 3, IC<3>(), BC<true>());
+    }
+    // (the products are asm: the wait states between the last and a read of
+    // its accumulators are ours to give, and the accumulators pass through
+    // what follows the wait, so that no read of them can stand before it)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("; accumulator complete" : "+a"(acc[i][j]));
+    __syncthreads();
+
+    // ---- epilogue: dst[m][n .. n+3] = acc (+ bias) in BF16.  The wave's 128
+    // tokens x 256 bytes go through its own region of LDS (chunk c of row r at
+    // c ^ (r & 15)), so that a store instruction writes four rows' 256 bytes.
+    // A wave touches only its own region (its LDS operations complete in order).
+    lds_t *const so = sbase + wave * 32768;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int n = n0 + 128 * wn + 16 * i + 4 * q4;
+        f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias && n < a.N) bias = *reinterpret_cast<const f32x4 *>(a.bias + n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const f32x4 v = acc[i][j] + bias;
+            *reinterpret_cast<__attribute__((address_space(3))) u32x2 *>(
+                so + (16 * j + l16) * 256 + (((2 * i + (q4 >> 1)) ^ l16) << 4) + ((q4 & 1) << 3)) =
+                (u32x2){Elem<__bf16>::pack2(v.x, v.y), Elem<__bf16>::pack2(v.z, v.w)};
+        }
+    }
+    typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));   // dst rows lie at multiples of 8 bytes
+    const int n = n0 + 128 * wn + 8 * l16;
+#pragma unroll
+    for (int t = 0; t < 32; ++t) {
+        const int r = 4 * t + q4, m = m0 + 128 * wm + r;
+        const u32x4 v = *reinterpret_cast<lds_u4 *>(so + r * 256 + ((l16 ^ (r & 15)) << 4));
+        char *const p = a.dst + (int64_t)m * a.d_nb1 + (int64_t)n * 2;
+        if (m < a.M) {
+            if (n + 8 <= a.N)
+                __builtin_nontemporal_store((u32x4_8)v, reinterpret_cast<u32x4_8 *>(p));
+            else if (n < a.N)
+                __builtin_nontemporal_store((u32x2){v.x, v.y}, reinterpret_cast<u32x2 *>(p));
+        }
+    }
+}
+
 template <int NB, int MB, int D>
 static void launch_stream(const F8MmArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((f8_mm_stream<NB, MB, D>), dim3(a.n_blocks), dim3(256), 0, s, a);
@@ -213,6 +475,7 @@ hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t s) {
     switch (tile) {
     case 401: launch_stream<4, 1, 4>(a, s); break;
     case 404: launch_stream<4, 4, 2>(a, s); break;
+    case 1616: hipLaunchKernelGGL(f8_mm_tile, dim3(a.n_blocks), dim3(256), 0, s, a); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

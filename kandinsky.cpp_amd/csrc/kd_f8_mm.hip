@@ -12,6 +12,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 #include "../../include/kd_f8.h"
 #include "kd_f8_kernel.h"
 #include "kd_fa_device.h"
@@ -28,6 +30,16 @@ static __device__ __forceinline__ f32x4 mfma_f8(i32x8 a, i32x8 b, f32x4 c, uint3
 
 static __device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
     return (i32x8){(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+}
+
+// f(IC<0>()) ... f(IC<N - 1>()): a loop that is unrolled whatever its size.
+template <class F, int... I>
+static __device__ __forceinline__ void static_for(F f, std::integer_sequence<int, I...>) {
+    (f(IC<I>()), ...);
+}
+template <int N, class F>
+static __device__ __forceinline__ void static_for(F f) {
+    static_for(f, std::make_integer_sequence<int, N>());
 }
 
 // The tile of a workgroup: XCD-contiguous runs, dealt in columns of `cols`
@@ -264,43 +276,58 @@ void f8_mm_tile(F8MmArgs a) {
     const int ng = (nk + 3) >> 2;                       // words of scales
 
     // DMA j of a wave: rows 8 (wave + 4 j) .. +7, lane l the chunk that lies
-    // at l % 8 of row l / 8
-    uint32_t w_off[8], x_off[8];
+    // at l % 8 of row l / 8.  Row offsets are made where they are used (a few
+    // instructions under a product), not kept in registers: `fresh` hides from
+    // the compiler that they are the same every time.
+    const int dr = 8 * wave + (lane >> 3);
     const int dc = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int r = 8 * (wave + 4 * j) + (lane >> 3);
-        w_off[j] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.w_nb1 + (uint32_t)(dc << 4);
-        x_off[j] = (uint32_t)min(r, a.M - 1 - m0) * (uint32_t)a.x_nb1 + (uint32_t)(dc << 4);
-    }
+    const int w_last = a.N - 1 - n0, x_last = a.M - 1 - m0;
+    auto fresh = [](int v) __attribute__((always_inline)) {
+        asm volatile("" : "+v"(v));
+        return v;
+    };
+    auto row_off = [](int r, int last, int64_t nb1) __attribute__((always_inline)) {
+        return __umul24((uint32_t)min(r, last), (uint32_t)nb1);   // (strides are below 2^24: kd_f8_host.cpp)
+    };
     const char *const wtile = a.w + (int64_t)n0 * a.w_nb1;
     const char *const xtile = a.x + (int64_t)m0 * a.x_nb1;
-    auto dma = [&](const char *tile, uint32_t off, int kt, lds_t *buf, int j, auto end_c) __attribute__((always_inline)) {
+    const char *const wst = a.ws + (int64_t)n0 * a.ws_nb1;
+    const char *const xst = a.xs + (int64_t)m0 * a.xs_nb1;
+    auto dma = [&](const char *tile, int last, int64_t nb1, int kt, lds_t *buf, int j, auto end_c) __attribute__((always_inline)) {
+        uint32_t off = row_off(fresh(dr) + 32 * j, last, nb1);
         int64_t k0 = (int64_t)kt * 128;
         if constexpr (decltype(end_c)::value) {
-            off = kt >= nk ? 0 : kt * 128 + 16 * dc < a.K ? off : off - (uint32_t)(dc << 4);
+            off = kt >= nk ? 0 : kt * 128 + 16 * dc < a.K ? off + (uint32_t)(dc << 4) : off;
             k0 = kt >= nk ? 0 : k0;
+        } else {
+            off += (uint32_t)(dc << 4);
         }
         dma16(tile + k0, off, buf + (wave + 4 * j) * 1024);
     };
     auto dma_w = [&](int kt, int buf, int j, auto end_c) __attribute__((always_inline)) {
-        dma(wtile, w_off[j], kt, sbase + buf * kTileBuf, j, end_c);
+        dma(wtile, w_last, a.w_nb1, kt, sbase + buf * kTileBuf, j, end_c);
     };
     auto dma_x = [&](int kt, int buf, int j, auto end_c) __attribute__((always_inline)) {
-        dma(xtile, x_off[j], kt, sbase + (2 + buf) * kTileBuf, j, end_c);
+        dma(xtile, x_last, a.x_nb1, kt, sbase + (2 + buf) * kTileBuf, j, end_c);
     };
 
-    // scales: row 16 i + l16 of this wave's half
-    uint32_t sw[8], sx[8], nw[8], nx[8];
-    auto load_scales = [&](int g) __attribute__((always_inline)) {
+    // scales: sw[i], sx[j] the words of row 16 i + l16 of this wave's halves.
+    // Lane l loads those of rows l and 64 + l, once each (a load of 16 rows by
+    // four lanes each takes the address unit as long); three swaps then give
+    // four fragments' words.
+    uint32_t sw[8], sx[8], nw[8], nx[8], raw[4];
+    auto load_scales = [&](int g, int q) __attribute__((always_inline)) {
         const int o = 4 * min(g, ng - 1);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t rn = (uint32_t)min(128 * wn + 16 * i + l16, a.N - 1 - n0) * (uint32_t)a.ws_nb1;
-            const uint32_t rm = (uint32_t)min(128 * wm + 16 * i + l16, a.M - 1 - m0) * (uint32_t)a.xs_nb1;
-            nw[i] = *reinterpret_cast<const uint32_t *>(a.ws + (int64_t)n0 * a.ws_nb1 + (uint64_t)(rn + o));
-            nx[i] = *reinterpret_cast<const uint32_t *>(a.xs + (int64_t)m0 * a.xs_nb1 + (uint64_t)(rm + o));
-        }
+        const bool w = q < 2;
+        const uint32_t r = row_off(fresh(lane) + (w ? 128 * wn : 128 * wm) + 64 * (q & 1), w ? w_last : x_last, w ? a.ws_nb1 : a.xs_nb1);
+        raw[q] = *reinterpret_cast<const uint32_t *>((w ? wst : xst) + (uint64_t)(r + o));
+    };
+    auto spread_scales = [&](int q) __attribute__((always_inline)) {
+        uint32_t *const to = (q < 2 ? nw : nx) + 4 * (q & 1);
+        const auto h = __builtin_amdgcn_permlane32_swap(raw[q], raw[q], false, false);
+        const auto u = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
+        const auto v = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+        to[0] = u[0]; to[1] = u[1]; to[2] = v[0]; to[3] = v[1];
     };
 
     // fragments
@@ -340,39 +367,40 @@ void f8_mm_tile(F8MmArgs a) {
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int p = 0; p < 64; ++p) {
-            const int i = p >> 3, j = p & 7;
-            if (p == 48) {
+        static_for<64>([&](auto p_c) __attribute__((always_inline)) {
+            constexpr int p = decltype(p_c)::value, i = p >> 3, j = p & 7;
+            if constexpr (p == 48) {
                 if constexpr (S == 3) {
                     // the next words of scales, loaded a step ago (the
                     // compiler waits for them here)
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) asm volatile("" : "+v"(nw[q]), "+v"(nx[q]));
+                    for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(raw[q]));
                 }
                 // all but the 8 DMAs of X of stage kt + 3 have landed
                 asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
                 __syncthreads();
-                if constexpr (S == 2) load_scales((kt >> 2) + 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             mfma_f8_asm<S>(acc[i][j], join(fw[i & 3][0], fw[i & 3][1]), join(fx[P][j][0], fx[P][j][1]), sw[i], sx[j]);
             __builtin_amdgcn_sched_barrier(0);
             // X of stage kt + 3, into the buffer that the last step freed
-            if (p < 32 && p % 4 == 0) dma_x(kt + 3, xprev, p / 4, end_c);
+            if constexpr (p < 32 && p % 4 == 0) dma_x(kt + 3, xprev, p / 4, end_c);
             // W's fragment two on
-            if (i < 6 && (j == 1 || j == 3)) read_w(P, i + 2, j >> 1);
+            if constexpr (i < 6 && (j == 1 || j == 3)) read_w(P, i + 2, j >> 1);
             // X of stage kt + 1
-            if (i < 4 && (j == 2 || j == 4 || j == 5 || j == 7)) {
-                const int q = 4 * i + (j == 2 ? 0 : j == 4 ? 1 : j == 5 ? 2 : 3);
+            if constexpr (i < 4 && (j == 2 || j == 4 || j == 5 || j == 7)) {
+                constexpr int q = 4 * i + (j == 2 ? 0 : j == 4 ? 1 : j == 5 ? 2 : 3);
                 read_x(xb, IC<1 - P>(), q >> 1, q & 1);
             }
-            if (p >= 48) {
-                if (j % 2 == 0) dma_w(kt + 2, P, (p - 48) / 2, end_c);
-                if (j == 1 || j == 3) read_w(1 - P, i - 6, j >> 1);
+            if constexpr (p >= 48) {
+                if constexpr (j % 2 == 0) dma_w(kt + 2, P, (p - 48) / 2, end_c);
+                if constexpr (j == 1 || j == 3) read_w(1 - P, i - 6, j >> 1);
+                // the next group's scales, ahead of W's last DMAs
+                if constexpr (S == 2 && p < 56 && j % 2 == 1) load_scales((kt >> 2) + 1, j >> 1);
+                if constexpr (S == 3 && j % 4 == 0) spread_scales((p - 48) >> 2);
             }
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
         xb = xb == 2 ? 0 : xb + 1;
         if constexpr (S == 3) {
 #pragma unroll
@@ -381,11 +409,16 @@ void f8_mm_tile(F8MmArgs a) {
         }
     };
 
-    load_scales(0);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) { sw[q] = nw[q]; sx[q] = nx[q]; }
+    for (int q = 0; q < 4; ++q) load_scales(0, q);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) asm volatile("" : "+v"(sw[q]), "+v"(sx[q]));
+    for (int q = 0; q < 4; ++q) spread_scales(q);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        sw[q] = nw[q];
+        sx[q] = nx[q];
+        asm volatile("" : "+v"(sw[q]), "+v"(sx[q]));
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) dma_x(0, 0, j, BC<true>());
 #pragma unroll

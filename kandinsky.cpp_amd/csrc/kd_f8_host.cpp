@@ -135,7 +135,7 @@ int validate(const kd_f8_mm_desc *d) {
         if (st != KD_FA_OK) return st;
     }
     // a tile's rows are addressed with 32-bit offsets from its first
-    for (const kd_fa_tensor *t : {&d->w.codes, &d->w.scales, &d->x.codes, &d->x.scales})
+    for (const kd_fa_tensor *t : {&d->w.codes, &d->w.scales, &d->x.codes, &d->x.scales, &o})
         if (flat_rows(*t) > 1 && (uint64_t)t->nb[1] > kU32Max / 256) return KD_FA_ERR_LAYOUT;
     return KD_FA_OK;
 }
@@ -233,7 +233,7 @@ int kd_f8_mm_run(const kd_f8_mm_desc *desc, void *stream) {
     a.xs_nb1 = (int64_t)desc->x.scales.nb[1];
     a.bias = static_cast<const float *>(desc->bias.data);
     a.dst = static_cast<char *>(desc->dst.data);
-    a.d_nb1 = (int64_t)desc->dst.nb[1];
+    a.d_nb1 = M > 1 ? (int64_t)desc->dst.nb[1] : N * 2;   // (one row's stride may be anything)
     a.M = (int32_t)M;
     a.N = (int32_t)N;
     a.K = (int32_t)K;

@@ -293,41 +293,61 @@ void f8_mm_tile(F8MmArgs a) {
     const char *const xtile = a.x + (int64_t)m0 * a.x_nb1;
     const char *const wst = a.ws + (int64_t)n0 * a.ws_nb1;
     const char *const xst = a.xs + (int64_t)m0 * a.xs_nb1;
-    auto dma = [&](const char *tile, int last, int64_t nb1, int kt, lds_t *buf, int j, auto end_c) __attribute__((always_inline)) {
-        uint32_t off = row_off(fresh(dr) + 32 * j, last, nb1);
-        int64_t k0 = (int64_t)kt * 128;
+    // Stage kt of W or X: its first byte of the tile's first row, the tile's
+    // last row and the lane's chunk.  A stage that is not there is the tile's
+    // first chunk for every lane, a chunk past K its row's first.
+    struct Stage { const char *at; int last; uint32_t chunk; };
+    auto stage = [&](const char *tile, int last, int kt, auto end_c) __attribute__((always_inline)) {
+        Stage t = {tile + (int64_t)kt * 128, last, (uint32_t)(dc << 4)};
         if constexpr (decltype(end_c)::value) {
-            off = kt >= nk ? 0 : kt * 128 + 16 * dc < a.K ? off + (uint32_t)(dc << 4) : off;
-            k0 = kt >= nk ? 0 : k0;
-        } else {
-            off += (uint32_t)(dc << 4);
+            t.chunk = kt * 128 + 16 * dc < a.K ? t.chunk : 0;
+            t.last = kt < nk ? last : 0;
+            t.at = kt < nk ? t.at : tile;
         }
-        dma16(tile + k0, off, buf + (wave + 4 * j) * 1024);
+        return t;
     };
-    auto dma_w = [&](int kt, int buf, int j, auto end_c) __attribute__((always_inline)) {
-        dma(wtile, w_last, a.w_nb1, kt, sbase + buf * kTileBuf, j, end_c);
+    auto dma_w = [&](const Stage &t, int buf, int j) __attribute__((always_inline)) {
+        dma16(t.at, row_off(fresh(dr) + 32 * j, t.last, a.w_nb1) + t.chunk, sbase + buf * kTileBuf + (wave + 4 * j) * 1024);
     };
-    auto dma_x = [&](int kt, int buf, int j, auto end_c) __attribute__((always_inline)) {
-        dma(xtile, x_last, a.x_nb1, kt, sbase + (2 + buf) * kTileBuf, j, end_c);
+    auto dma_x = [&](const Stage &t, int buf, int j) __attribute__((always_inline)) {
+        dma16(t.at, row_off(fresh(dr) + 32 * j, t.last, a.x_nb1) + t.chunk, sbase + (2 + buf) * kTileBuf + (wave + 4 * j) * 1024);
     };
 
     // scales: sw[i], sx[j] the words of row 16 i + l16 of this wave's halves.
-    // Lane l loads those of rows l and 64 + l, once each (a load of 16 rows by
-    // four lanes each takes the address unit as long); three swaps then give
-    // four fragments' words.
-    uint32_t sw[8], sx[8], nw[8], nx[8], raw[4];
-    auto load_scales = [&](int g, int q) __attribute__((always_inline)) {
-        const int o = 4 * min(g, ng - 1);
-        const bool w = q < 2;
-        const uint32_t r = row_off(fresh(lane) + (w ? 128 * wn : 128 * wm) + 64 * (q & 1), w ? w_last : x_last, w ? a.ws_nb1 : a.xs_nb1);
-        raw[q] = *reinterpret_cast<const uint32_t *>((w ? wst : xst) + (uint64_t)(r + o));
+    // Lane l loads those of rows l and 64 + l, once each and four words (16
+    // stages) at a time; three swaps then give four fragments' words.  (A
+    // load's lines are what it costs: each is 128 bytes out of the L2.  Rows
+    // loaded by four lanes each 1.03 -> 0.88 ms at 63,488 x 4096 x 4096.)
+    typedef uint32_t u32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
+    uint32_t sw[8], sx[8], nw[8], nx[8];
+    u32x4 raw[4];
+    auto load_scales = [&](int b) __attribute__((always_inline)) {   // words 4 b .. +3
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const bool w = q < 2;
+            const uint32_t r = row_off(fresh(lane) + (w ? 128 * wn : 128 * wm) + 64 * (q & 1), w ? w_last : x_last, w ? a.ws_nb1 : a.xs_nb1);
+            const char *const row = (w ? wst : xst) + (uint64_t)r;
+            if (4 * b + 4 <= ng) {
+                raw[q] = *reinterpret_cast<const u32x4_4 *>(row + 16 * b);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) raw[q][e] = *reinterpret_cast<const uint32_t *>(row + 4 * min(4 * b + e, ng - 1));
+            }
+        }
     };
+    // the next word of rows q
     auto spread_scales = [&](int q) __attribute__((always_inline)) {
         uint32_t *const to = (q < 2 ? nw : nx) + 4 * (q & 1);
-        const auto h = __builtin_amdgcn_permlane32_swap(raw[q], raw[q], false, false);
+        const auto h = __builtin_amdgcn_permlane32_swap(raw[q].x, raw[q].x, false, false);
         const auto u = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
         const auto v = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
         to[0] = u[0]; to[1] = u[1]; to[2] = v[0]; to[3] = v[1];
+        raw[q] = (u32x4){raw[q].y, raw[q].z, raw[q].w, raw[q].w};
+    };
+    auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { sw[q] = nw[q]; sx[q] = nx[q]; }
+        asm volatile("s_nop 4" ::: "memory");   // (the products are asm: VALU results before they read them)
     };
 
     // fragments
@@ -354,6 +374,7 @@ void f8_mm_tile(F8MmArgs a) {
         constexpr int S = decltype(sel_c)::value, P = S & 1;
         constexpr bool END = decltype(end_c)::value;
         const int xprev = xb == 0 ? 2 : xb - 1;   // freed by the last step's barrier
+        const Stage next_w = stage(wtile, w_last, kt + 2, end_c), next_x = stage(xtile, x_last, kt + 3, end_c);
         if constexpr (END) {
             if (kt >= whole) {
                 // the one stage that ends inside: what lies past K is zero
@@ -384,7 +405,7 @@ void f8_mm_tile(F8MmArgs a) {
             mfma_f8_asm<S>(acc[i][j], join(fw[i & 3][0], fw[i & 3][1]), join(fx[P][j][0], fx[P][j][1]), sw[i], sx[j]);
             __builtin_amdgcn_sched_barrier(0);
             // X of stage kt + 3, into the buffer that the last step freed
-            if constexpr (p < 32 && p % 4 == 0) dma_x(kt + 3, xprev, p / 4, end_c);
+            if constexpr (p < 32 && p % 4 == 0) dma_x(next_x, xprev, p / 4);
             // W's fragment two on
             if constexpr (i < 6 && (j == 1 || j == 3)) read_w(P, i + 2, j >> 1);
             // X of stage kt + 1
@@ -393,42 +414,36 @@ void f8_mm_tile(F8MmArgs a) {
                 read_x(xb, IC<1 - P>(), q >> 1, q & 1);
             }
             if constexpr (p >= 48) {
-                if constexpr (j % 2 == 0) dma_w(kt + 2, P, (p - 48) / 2, end_c);
+                if constexpr (j % 2 == 0) dma_w(next_w, P, (p - 48) / 2);
                 if constexpr (j == 1 || j == 3) read_w(1 - P, i - 6, j >> 1);
-                // the next group's scales, ahead of W's last DMAs
-                if constexpr (S == 2 && p < 56 && j % 2 == 1) load_scales((kt >> 2) + 1, j >> 1);
+                // the next four groups' scales, ahead of W's last DMAs
+                if constexpr (S == 2 && p == 49) {
+                    if (((kt >> 2) & 3) == 3) load_scales(((kt >> 2) + 1) >> 2);
+                }
                 if constexpr (S == 3 && j % 4 == 0) spread_scales((p - 48) >> 2);
             }
             __builtin_amdgcn_sched_barrier(0);
         });
         xb = xb == 2 ? 0 : xb + 1;
-        if constexpr (S == 3) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) { sw[q] = nw[q]; sx[q] = nx[q]; }
-            asm volatile("s_nop 4" ::: "memory");
-        }
+        if constexpr (S == 3) take_scales();
     };
 
+    load_scales(0);
+    {
+        const Stage x0 = stage(xtile, x_last, 0, BC<true>()), w0 = stage(wtile, w_last, 0, BC<true>()),
+                    x1 = stage(xtile, x_last, 1, BC<true>()), w1 = stage(wtile, w_last, 1, BC<true>()),
+                    x2 = stage(xtile, x_last, 2, BC<true>());
 #pragma unroll
-    for (int q = 0; q < 4; ++q) load_scales(0, q);
+        for (int j = 0; j < 8; ++j) dma_x(x0, 0, j);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) spread_scales(q);
+        for (int j = 0; j < 8; ++j) dma_w(w0, 0, j);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        sw[q] = nw[q];
-        sx[q] = nx[q];
-        asm volatile("" : "+v"(sw[q]), "+v"(sx[q]));
+        for (int j = 0; j < 8; ++j) dma_x(x1, 1, j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dma_w(w1, 1, j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dma_x(x2, 2, j);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dma_x(0, 0, j, BC<true>());
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dma_w(0, 0, j, BC<true>());
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dma_x(1, 1, j, BC<true>());
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dma_w(1, 1, j, BC<true>());
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dma_x(2, 2, j, BC<true>());
     asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
     __syncthreads();
 #pragma unroll
@@ -439,6 +454,9 @@ void f8_mm_tile(F8MmArgs a) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) read_w(0, i, h);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) spread_scales(q);
+    take_scales();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();
 

@@ -159,7 +159,7 @@ int launched(hipError_t e) { return e == hipSuccess ? KD_FA_OK : KD_FA_ERR_LAUNC
 
 int choose_tile(int64_t M, int64_t N, int64_t K) {
     (void)N; (void)K;
-    return M <= 16 ? 401 : M < 256 ? 404 : 1616;
+    return M <= 16 ? 401 : M < 64 ? 202 : M < 512 ? 405 : M < 3000 ? 10810 : 11616;
 }
 
 }  // namespace
@@ -217,7 +217,7 @@ int kd_f8_mm_run(const kd_f8_mm_desc *desc, void *stream) {
     const int64_t K = desc->w.codes.ne[0], N = desc->w.codes.ne[1], M = flat_rows(desc->x.codes);
     if (M == 0 || N == 0) return KD_FA_OK;
     const int tile = choose_tile(M, N, K);
-    const int64_t tn = 16 * (tile / 100), tm = 16 * (tile % 100);
+    const int64_t tn = 16 * (tile / 100 % 100), tm = 16 * (tile % 100);
     const int64_t tiles_n = (N + tn - 1) / tn, tiles_m = (M + tm - 1) / tm;
     if (tiles_n * tiles_m > kdfa::kF8MmMaxBlocks) return KD_FA_ERR_SHAPE;
     st = kdfa::device_gfx950();

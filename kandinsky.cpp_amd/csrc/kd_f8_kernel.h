@@ -40,7 +40,8 @@ struct F8MmArgs {
 };
 
 constexpr int64_t kF8MmMaxBlocks = 1 << 23;   // workgroups of 256 threads in one launch, with room to spare
-// Tiles of 16 * (tile / 100) outputs x 16 * (tile % 100) tokens.
+// Tiles of 16 * (tile / 100 % 100) outputs x 16 * (tile % 100) tokens: below
+// 10000 f8_mm_ring's, above f8_mm_grid's, 11616 f8_mm_tile's.
 hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t stream);
 
 }  // namespace kdfa

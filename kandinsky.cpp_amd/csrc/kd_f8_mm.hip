@@ -22,10 +22,16 @@ namespace kdfa {
 
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 
-// D += A B, each row's codes times the scale in byte SEL of its word
-template <int SEL>
+// D += A B, each row's codes times the scale in byte 0 of its word
 static __device__ __forceinline__ f32x4 mfma_f8(i32x8 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, SEL, (int)sa, SEL, (int)sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
+}
+
+// A DMA of one word per lane, each lane its own address, into 256 bytes of
+// LDS (as dma16: every consumer waits with an explicit s_waitcnt vmcnt).
+static __device__ __forceinline__ void dma4(const char *p, lds_t *lds_wave_base) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_wave_base);
+    asm volatile("global_load_lds_dword %0, off" :: "v"(p), "{m0}"(m0));
 }
 
 static __device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
@@ -55,20 +61,57 @@ static __device__ __forceinline__ void f8_tile(const F8MmArgs &a, int &nt, int &
     nt = col * a.cols + rem - mt * width;
 }
 
+// A wave's part of dst out of LDS: R rows of C chunks of 16 bytes, chunk c of
+// row r at c ^ swz(r), to tokens m0 .. and outputs n0 ..
+template <int R, int C, class Swz>
+static __device__ __forceinline__ void store_rows(const F8MmArgs &a, const lds_t *from, Swz swz, int m0, int n0, int lane) {
+    typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));   // dst rows lie at multiples of 8 bytes
+    const int c = lane % C, n = n0 + 8 * c;
+#pragma unroll
+    for (int t = 0; t < R * C / 64; ++t) {
+        const int r = t * (64 / C) + lane / C, m = m0 + r;
+        const u32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4 *>(from + r * (16 * C) + ((c ^ swz(r)) << 4));
+        char *const p = a.dst + (int64_t)m * a.d_nb1 + (int64_t)n * 2;
+        if (m < a.M) {
+            if (n + 8 <= a.N)
+                __builtin_nontemporal_store((u32x4_8)v, reinterpret_cast<u32x4_8 *>(p));
+            else if (n < a.N)
+                __builtin_nontemporal_store((u32x2){v.x, v.y}, reinterpret_cast<u32x2 *>(p));
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------
-// f8_mm_stream: 16 NB outputs x 16 MB tokens per workgroup, the four waves
-// splitting k (whole words of scales, 512 k, each).  A wave computes the
-// whole tile over its own k, so nothing that it loads is another wave's: the
-// rows go from memory straight into registers, D blocks ahead.  The four
-// partial sums meet in LDS, in wave order.
-// Rows past N or M are the last row again (not stored); k past K reads the
-// row's last 16 bytes, X's then zeroed.
+// f8_mm_ring: 16 NB outputs x 16 MB tokens per workgroup, for calls of few
+// tokens or few tiles.  The four waves split k, each a run of stages of 128 k,
+// and compute the whole tile over it: nothing that a wave loads is another's,
+// so each keeps its own ring of S stages in LDS, filled by DMA, and no barrier
+// stands before the four partial sums meet, in wave order.  A stage's
+// fragments go into registers at once, and its buffer to stage S on: what is
+// on its way is the whole of LDS, whatever the tile.
+//
+// The scales of a run (of 32 stages of it, if it is longer) are brought ahead
+// of its first stage, row by row in words, and read a byte at a time.
+// In LDS 16-byte chunk c of row r lies at c ^ ((r >> 1) & 7).  Rows past N or
+// M are the last row again (not stored); a chunk past K is its row's first of
+// the stage, X's then zeroed in the registers.
 // ---------------------------------------------------------------------------
-template <int NB, int MB, int D>
-__global__ __launch_bounds__(256) void f8_mm_stream(F8MmArgs a) {
-    constexpr int PN = NB * MB <= 16 ? NB : 16 / MB;   // fragments of outputs that are joined at once
+constexpr int kRingWords = 8;   // words of scales per row at a time
+
+template <int NB, int MB, int S>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
+void f8_mm_ring(F8MmArgs a) {
+    constexpr int kRows = 16 * (NB + MB);
+    constexpr int kStage = kRows * 128;
+    constexpr int kDma = kRows / 8;                         // of a stage
+    constexpr int kWordRows = (kRows + 63) / 64 * 64;       // rows of a word's DMAs
+    constexpr int kScales = kRingWords * kWordRows * 4;
+    constexpr int kWave = S * kStage + kScales;
+    constexpr int PN = NB % 4 == 0 ? 4 : NB % 2 == 0 ? 2 : 1;   // fragments of outputs that are joined at once
     constexpr int kPart = 16 * MB * 16 * PN * 4;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kPart];
+    constexpr int kLds = 4 * (kWave > kPart ? kWave : kPart);
+    static_assert(kLds <= 163840 && (S - 1) * kDma <= 63, "LDS, and the counter of what is on its way");
+    __shared__ __attribute__((aligned(1024))) char lds[kLds];
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -77,120 +120,113 @@ __global__ __launch_bounds__(256) void f8_mm_stream(F8MmArgs a) {
     int nt, mt;
     f8_tile(a, nt, mt);
     const int n0 = nt * (16 * NB), m0 = mt * (16 * MB);
-
-    uint32_t w_off[NB], x_off[MB], ws_off[NB], xs_off[MB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const uint32_t r = (uint32_t)min(16 * i + l16, a.N - 1 - n0);
-        w_off[i] = r * (uint32_t)a.w_nb1;
-        ws_off[i] = r * (uint32_t)a.ws_nb1;
-    }
-#pragma unroll
-    for (int j = 0; j < MB; ++j) {
-        const uint32_t r = (uint32_t)min(16 * j + l16, a.M - 1 - m0);
-        x_off[j] = r * (uint32_t)a.x_nb1;
-        xs_off[j] = r * (uint32_t)a.xs_nb1;
-    }
+    const int w_last = a.N - 1 - n0, x_last = a.M - 1 - m0;
     const char *const wt = a.w + (int64_t)n0 * a.w_nb1;
     const char *const xt = a.x + (int64_t)m0 * a.x_nb1;
-    const char *const wst = a.ws + (int64_t)n0 * a.ws_nb1;
-    const char *const xst = a.xs + (int64_t)m0 * a.xs_nb1;
+    lds_t *const ring = LDS_PTR(char, lds) + wave * kWave;
+    lds_t *const words = ring + S * kStage;
 
-    // this wave's groups of four blocks
-    const int ng = (int)(((uint32_t)a.K + 511) >> 9);
-    const int g0 = (int)((int64_t)wave * ng >> 2), g1 = (int)((int64_t)(wave + 1) * ng >> 2);
+    // DMA j of a stage: rows 8 j .. +7 (W's, then X's), lane l the chunk that
+    // lies at l % 8 of row l / 8
+    uint32_t off[kDma];
+#pragma unroll
+    for (int j = 0; j < kDma; ++j) {
+        const int r = 8 * j + (lane >> 3);
+        off[j] = j < 2 * NB ? (uint32_t)min(r, w_last) * (uint32_t)a.w_nb1 : (uint32_t)min(r - 16 * NB, x_last) * (uint32_t)a.x_nb1;
+    }
+    const int c0 = (lane & 7) ^ (lane >> 4), c1 = c0 ^ 4;   // chunks of even and odd j
+    const int nk = (int)(((uint32_t)a.K + 127) >> 7);
+    // this wave's stages
+    const int k0 = (int)((int64_t)wave * nk >> 2), k1 = (int)((int64_t)(wave + 1) * nk >> 2);
+    // stage kt into ring buffer buf; past this wave's last, the tile's first
+    // chunk for every lane (not used), so that the counter counts alike
+    auto issue = [&](int kt, int buf) __attribute__((always_inline)) {
+        lds_t *const to = ring + buf * kStage;
+        if (kt < k1) {
+            const int64_t kb = (int64_t)kt * 128;
+            const int left = a.K - kt * 128;
+            const uint32_t b0 = 16 * c0 < left ? 16 * c0 : 0, b1 = 16 * c1 < left ? 16 * c1 : 0;
+#pragma unroll
+            for (int j = 0; j < kDma; ++j) dma16((j < 2 * NB ? wt : xt) + kb, off[j] + (j & 1 ? b1 : b0), to + j * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kDma; ++j) dma16(j < 2 * NB ? wt : xt, 0, to + j * 1024);
+        }
+    };
+    // words first .. +count-1 of the tile's rows, [word][row]
+    auto issue_words = [&](int first, int count) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < kWordRows / 64; ++h) {
+            // a lane's row: W's, then X's, then X's last again
+            const int r = 64 * h + lane, rx = r - 16 * NB;
+            const bool w = rx < 0;
+            const char *const p = w ? a.ws + (int64_t)(n0 + min(r, w_last)) * a.ws_nb1 : a.xs + (int64_t)(m0 + min(min(rx, 16 * MB - 1), x_last)) * a.xs_nb1;
+            for (int c = 0; c < count; ++c) dma4(p + 4 * (int64_t)(first + c), words + c * kWordRows * 4 + h * 256);
+        }
+    };
 
     f32x4 acc[NB][MB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int j = 0; j < MB; ++j) acc[i][j] = (f32x4){};
-    u32x4 fw[D][NB][2], fx[D][MB][2];
-    auto load = [&](int kt, auto d_c) __attribute__((always_inline)) {
-        constexpr int d = decltype(d_c)::value;
-        const uint32_t k0 = min((uint32_t)kt * 128 + 16 * q4, (uint32_t)a.K - 16);
-        const uint32_t k1 = min((uint32_t)kt * 128 + 16 * q4 + 64, (uint32_t)a.K - 16);
+    typedef const __attribute__((address_space(3))) u32x4 lds_u4;
+    const uint32_t f_rd = (uint32_t)(l16 * 128 + ((q4 ^ ((l16 >> 1) & 7)) << 4));
+    for (int ka = k0; ka < k1;) {   // runs of up to kRingWords words
+        const int first = ka >> 2, kb = min(k1, 4 * (first + kRingWords));
+        issue_words(first, ((kb + 3) >> 2) - first);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            fw[d][i][0] = ld16(wt + (uint64_t)(w_off[i] + k0));
-            fw[d][i][1] = ld16(wt + (uint64_t)(w_off[i] + k1));
-        }
+        for (int s = 0; s < S; ++s) issue(ka + s, s);
+        int buf = 0;
+        for (int kt = ka; kt < kb; ++kt) {
+            asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1) * kDma) : "memory");
+            const lds_t *const from = ring + buf * kStage;
+            u32x4 fw[NB][2], fx[MB][2];
+            uint32_t sw[NB], sx[MB];
+            const lds_t *const sp = words + ((kt >> 2) - first) * kWordRows * 4 + (kt & 3) + l16 * 4;
 #pragma unroll
-        for (int j = 0; j < MB; ++j) {
-            fx[d][j][0] = ld16(xt + (uint64_t)(x_off[j] + k0));
-            fx[d][j][1] = ld16(xt + (uint64_t)(x_off[j] + k1));
-        }
-    };
-    uint32_t sw[NB], sx[MB], nw[NB], nx[MB];
-    auto load_scales = [&](int g) __attribute__((always_inline)) {
-        const uint32_t o = (uint32_t)min(g, ng - 1) * 4;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) nw[i] = *reinterpret_cast<const uint32_t *>(wst + (uint64_t)(ws_off[i] + o));
-#pragma unroll
-        for (int j = 0; j < MB; ++j) nx[j] = *reinterpret_cast<const uint32_t *>(xst + (uint64_t)(xs_off[j] + o));
-    };
-    // the products of block kt (byte s of the scales' words)
-    auto products = [&](int kt, auto s_c, auto end_c) __attribute__((always_inline)) {
-        constexpr int s = decltype(s_c)::value, d = s % D;
-        // past K the scales' bytes are anything, NaN too
-        if (decltype(end_c)::value && kt * 128 >= a.K) return;
-        i32x8 b[MB];
-#pragma unroll
-        for (int j = 0; j < MB; ++j) {
-            u32x4 lo = fx[d][j][0], hi = fx[d][j][1];
-            if constexpr (decltype(end_c)::value) {
-                const int left = a.K - kt * 128 - 16 * q4;   // > 0: chunk q4 is a part of the row
-                lo = left > 0 ? lo : (u32x4){};
-                hi = left > 64 ? hi : (u32x4){};
+            for (int i = 0; i < NB; ++i) {
+                sw[i] = *reinterpret_cast<const __attribute__((address_space(3))) uint8_t *>(sp + 64 * i);
+                fw[i][0] = *reinterpret_cast<lds_u4 *>(from + f_rd + i * 2048);
+                fw[i][1] = *reinterpret_cast<lds_u4 *>(from + (f_rd ^ 64) + i * 2048);
             }
-            b[j] = join(lo, hi);
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+                sx[j] = *reinterpret_cast<const __attribute__((address_space(3))) uint8_t *>(sp + 64 * (NB + j));
+                fx[j][0] = *reinterpret_cast<lds_u4 *>(from + f_rd + (NB + j) * 2048);
+                fx[j][1] = *reinterpret_cast<lds_u4 *>(from + (f_rd ^ 64) + (NB + j) * 2048);
+            }
+            // the buffer is free when its reads have returned
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            issue(kt + S, buf);
+            buf = buf == S - 1 ? 0 : buf + 1;
+            if (kt * 128 + 128 > a.K) {
+                const int left = a.K - kt * 128 - 16 * q4;
+#pragma unroll
+                for (int j = 0; j < MB; ++j) {
+                    fx[j][0] = left > 0 ? fx[j][0] : (u32x4){};
+                    fx[j][1] = left > 64 ? fx[j][1] : (u32x4){};
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int j = 0; j < MB; ++j)
+                    acc[i][j] = mfma_f8(join(fw[i][0], fw[i][1]), join(fx[j][0], fx[j][1]), acc[i][j], sw[i], sx[j]);
         }
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const i32x8 w = join(fw[d][i][0], fw[d][i][1]);
-#pragma unroll
-            for (int j = 0; j < MB; ++j) acc[i][j] = mfma_f8<s>(w, b[j], acc[i][j], sw[i], sx[j]);
-        }
-    };
-    auto group = [&](int g, auto end_c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NB; ++i) sw[i] = nw[i];
-#pragma unroll
-        for (int j = 0; j < MB; ++j) sx[j] = nx[j];
-        load_scales(g + 1);
-        products(4 * g, IC<0>(), end_c);
-        load(4 * g + D, IC<0>());
-        products(4 * g + 1, IC<1>(), end_c);
-        load(4 * g + 1 + D, IC<1 % D>());
-        products(4 * g + 2, IC<2>(), end_c);
-        load(4 * g + 2 + D, IC<2 % D>());
-        products(4 * g + 3, IC<3>(), end_c);
-        load(4 * g + 3 + D, IC<3 % D>());
-    };
-    static_assert(D == 1 || D == 2 || D == 4, "a block's registers by its byte");
-    if (g0 < g1) {
-        load_scales(g0);
-        load(4 * g0, IC<0>());
-        if constexpr (D > 1) load(4 * g0 + 1, IC<1 % D>());
-        if constexpr (D > 2) {
-            load(4 * g0 + 2, IC<2 % D>());
-            load(4 * g0 + 3, IC<3 % D>());
-        }
-        // the last group may end inside a block, or before one
-        const int whole = (a.K & 511) == 0 ? g1 : min(g1, ng - 1);
-        int g = g0;
-        for (; g < whole; ++g) group(g, BC<false>());
-        if (g < g1) group(g, BC<true>());
+        // what is still on its way is the next run's (or nobody's)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        ka = kb;
     }
 
     // ---- the four partial sums, 16 PN outputs of every token at a time: row
     // m of 64 PN bytes, 16-byte chunk c at c ^ its swizzle
     lds_t *const sp = LDS_PTR(char, lds);
     constexpr int kChunks = 4 * PN;
-    auto swz = [](int m) { return PN == 1 ? (m >> 2) & 3 : PN == 2 ? (m >> 1) & 7 : m & (kChunks - 1); };
+    auto swz = [](int m) { return PN == 1 ? (m >> 2) & 3 : PN == 2 ? (m >> 1) & 7 : m & 15; };
 #pragma unroll
     for (int p = 0; p < NB / PN; ++p) {
-        if (p) __syncthreads();
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < PN; ++i)
 #pragma unroll
@@ -214,6 +250,215 @@ __global__ __launch_bounds__(256) void f8_mm_stream(F8MmArgs a) {
             __builtin_nontemporal_store(o, reinterpret_cast<u32x2 *>(a.dst + (int64_t)(m0 + m) * a.d_nb1 + (int64_t)n * 2));
         }
     }
+}
+
+// ---------------------------------------------------------------------------
+// f8_mm_grid: 32 NB outputs x 32 MB tokens per workgroup, its four waves a 2 x
+// 2 grid of 16 NB x 16 MB each: for calls whose 256 x 256 tiles would leave
+// CUs idle, and whose tiles of f8_mm_ring (where a wave holds the whole tile's
+// sums) would have to be so small that W and X come too often.
+//
+// S stages of 128 k in LDS, one barrier a step: step kt publishes stage kt + 1
+// -- behind the barrier every wave's reads of stage kt have returned -- reads
+// its fragments into the other set, and sends stage kt + S into stage kt's
+// buffer while the products of stage kt run.  Words of scales come ahead of
+// each fourth stage, into one of two slots.  LDS rows, rows past N or M and k
+// past K are f8_mm_ring's; a stage past the last is the tile's first chunk for
+// every lane, so that the counter counts alike.
+// ---------------------------------------------------------------------------
+template <int NB, int MB, int S>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
+void f8_mm_grid(F8MmArgs a) {
+    constexpr int kRows = 32 * (NB + MB);
+    constexpr int kStage = kRows * 128;
+    constexpr int kDma = NB + MB;                     // of a wave and stage
+    constexpr int kWordDma = (kRows + 255) / 256;     // of a wave and word
+    constexpr int kSlot = kWordDma * 1024;
+    constexpr int kWaveOut = 16 * MB * 32 * NB;       // a wave's part of dst
+    constexpr int kUse = S * kStage + 2 * kSlot;
+    constexpr int kLds = kUse > 4 * kWaveOut ? kUse : 4 * kWaveOut;
+    static_assert(kLds <= 163840 && S >= 2 && S <= 8, "LDS, and a slot of words that is read before it is written again");
+    __shared__ __attribute__((aligned(1024))) char lds[kLds];
+    lds_t *const sbase = LDS_PTR(char, lds);
+    lds_t *const words = sbase + S * kStage;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15;
+    const int q4 = lane >> 4;
+    const int wn = wave & 1, wm = wave >> 1;
+    int nt, mt;
+    f8_tile(a, nt, mt);
+    const int n0 = nt * (32 * NB), m0 = mt * (32 * MB);
+    const int w_last = a.N - 1 - n0, x_last = a.M - 1 - m0;
+    const char *const wt = a.w + (int64_t)n0 * a.w_nb1;
+    const char *const xt = a.x + (int64_t)m0 * a.x_nb1;
+    const int nk = (int)(((uint32_t)a.K + 127) >> 7);   // stages
+    const int whole = a.K >> 7;                         // those of 128 k
+    const int ng = (nk + 3) >> 2;                       // words of scales
+
+    // DMA j of a wave: rows 8 (wave + 4 j) .. +7 of W, then of X; lane l the
+    // chunk that lies at l % 8 of row l / 8
+    uint32_t off[kDma];
+    const int dc = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+#pragma unroll
+    for (int j = 0; j < kDma; ++j) {
+        const int r = 8 * (wave + 4 * j) + (lane >> 3);
+        off[j] = j < NB ? (uint32_t)min(r, w_last) * (uint32_t)a.w_nb1 : (uint32_t)min(r - 32 * NB, x_last) * (uint32_t)a.x_nb1;
+    }
+    // DMA h of a word: rows 256 h + 64 wave + lane (W's, X's, X's last again)
+    const char *word_at[kWordDma];
+#pragma unroll
+    for (int h = 0; h < kWordDma; ++h) {
+        const int r = 256 * h + 64 * wave + lane, rx = r - 32 * NB;
+        word_at[h] = rx < 0 ? a.ws + (int64_t)(n0 + min(r, w_last)) * a.ws_nb1
+                            : a.xs + (int64_t)(m0 + min(min(rx, 32 * MB - 1), x_last)) * a.xs_nb1;
+    }
+    // DMA j of stage kt, its words before its first
+    auto dma_j = [&](int kt, int buf, int j, auto word_c, auto end_c) __attribute__((always_inline)) {
+        if constexpr (decltype(word_c)::value) {
+            if (j == 0) {
+                const int g = min(kt >> 2, ng - 1);
+#pragma unroll
+                for (int h = 0; h < kWordDma; ++h) dma4(word_at[h] + 4 * (int64_t)g, words + ((kt >> 2) & 1) * kSlot + h * 1024 + wave * 256);
+            }
+        }
+        const char *at = (j < NB ? wt : xt) + (int64_t)kt * 128;
+        uint32_t o = off[j] + (uint32_t)(dc << 4);
+        if constexpr (decltype(end_c)::value) {
+            o = kt >= nk ? 0 : kt * 128 + 16 * dc < a.K ? o : off[j];
+            at = kt >= nk ? (j < NB ? wt : xt) : at;
+        }
+        dma16(at, o, sbase + buf * kStage + (wave + 4 * j) * 1024);
+    };
+
+    f32x4 acc[NB][MB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j) acc[i][j] = (f32x4){};
+    typedef const __attribute__((address_space(3))) u32x4 lds_u4;
+    typedef const __attribute__((address_space(3))) uint32_t lds_u1;
+    const uint32_t f_rd = (uint32_t)(l16 * 128 + ((q4 ^ ((l16 >> 1) & 7)) << 4));
+    const uint32_t w_rd = f_rd + 16 * NB * wn * 128, x_rd = f_rd + (32 * NB + 16 * MB * wm) * 128;
+    u32x4 fw[2][NB][2], fx[2][MB][2];
+    uint32_t sw[NB], sx[MB], nw[NB], nx[MB];
+    auto read = [&](int buf, auto set_c) __attribute__((always_inline)) {
+        constexpr int set = decltype(set_c)::value;
+        const lds_t *const from = sbase + buf * kStage;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) fw[set][i][h] = *reinterpret_cast<lds_u4 *>(from + (w_rd ^ (h << 6)) + i * 2048);
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) fx[set][j][h] = *reinterpret_cast<lds_u4 *>(from + (x_rd ^ (h << 6)) + j * 2048);
+    };
+    auto read_words = [&](int g) __attribute__((always_inline)) {
+        const lds_t *const from = words + (g & 1) * kSlot + l16 * 4;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) nw[i] = *reinterpret_cast<lds_u1 *>(from + (16 * NB * wn + 16 * i) * 4);
+#pragma unroll
+        for (int j = 0; j < MB; ++j) nx[j] = *reinterpret_cast<lds_u1 *>(from + (32 * NB + 16 * MB * wm + 16 * j) * 4);
+    };
+    // operations behind stage s + 1's, when stages up to s + S - 1 are issued
+    // (s as far as it counts: its place in a group of four)
+    auto later = [](int s, int from) constexpr {
+        int n = 0;
+        for (int t = s + from; t < s + S; ++t) n += kDma + (t % 4 == 0 ? kWordDma : 0);
+        return n;
+    };
+
+    int buf = 0;   // of stage kt
+    auto step = [&](int kt, auto sel_c, auto end_c) __attribute__((always_inline)) {
+        constexpr int Q = decltype(sel_c)::value, P = Q & 1;
+        const int here = buf;
+        buf = buf == S - 1 ? 0 : buf + 1;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(later(Q, 2)) : "memory");
+        __syncthreads();
+        read(buf, IC<1 - P>());
+        if constexpr (Q == 3) read_words((kt >> 2) + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (decltype(end_c)::value) {
+            if (kt >= whole) {
+                const int left = a.K - kt * 128 - 16 * q4;
+#pragma unroll
+                for (int j = 0; j < MB; ++j) {
+                    fx[P][j][0] = left > 0 ? fx[P][j][0] : (u32x4){};
+                    fx[P][j][1] = left > 64 ? fx[P][j][1] : (u32x4){};
+                }
+            }
+        }
+        static_for<NB * MB>([&](auto p_c) __attribute__((always_inline)) {
+            constexpr int p = decltype(p_c)::value, i = p / MB, j = p % MB;
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(fw[P][i][0], fw[P][i][1]), join(fx[P][j][0], fx[P][j][1]), acc[i][j],
+                                                                         0, 0, Q, (int)sw[i], Q, (int)sx[j]);
+            __builtin_amdgcn_sched_barrier(0);
+            static_for<kDma>([&](auto d_c) __attribute__((always_inline)) {
+                constexpr int d = decltype(d_c)::value;
+                if constexpr (d * (NB * MB) / kDma == p) dma_j(kt + S, here, d, BC<(Q + S) % 4 == 0>(), end_c);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (Q == 3) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) sw[i] = nw[i];
+#pragma unroll
+            for (int j = 0; j < MB; ++j) sx[j] = nx[j];
+        }
+    };
+
+    static_for<S>([&](auto s_c) __attribute__((always_inline)) {
+        constexpr int s = decltype(s_c)::value;
+#pragma unroll
+        for (int j = 0; j < kDma; ++j) dma_j(s, s, j, BC<s % 4 == 0>(), BC<true>());
+    });
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(later(0, 1)) : "memory");
+    __syncthreads();
+    read(0, IC<0>());
+    read_words(0);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) sw[i] = nw[i];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) sx[j] = nx[j];
+    int kt = 0;
+    for (; kt + 3 + S < whole; kt += 4) {   // the last step's DMAs are of stage kt + 3 + S
+        step(kt, IC<0>(), BC<false>());
+        step(kt + 1, IC<1>(), BC<false>());
+        step(kt + 2, IC<2>(), BC<false>());
+        step(kt + 3, IC<3>(), BC<false>());
+    }
+    for (; kt < nk; kt += 4) {
+        step(kt, IC<0>(), BC<true>());
+        if (kt + 1 < nk) step(kt + 1, IC<1>(), BC<true>());
+        if (kt + 2 < nk) step(kt + 2, IC<2>(), BC<true>());
+        if (kt + 3 < nk) step(kt + 3, IC<3>(), BC<true>());
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+
+    // ---- dst[m][n .. n+3] = acc (+ bias) in BF16, through the wave's own
+    // region of LDS (its operations complete in order): rows of 32 NB bytes,
+    // 16-byte chunk c of row r at c ^ swz(r), stored as whole rows
+    constexpr int kC = 2 * NB;
+    auto swz = [](int r) { return (r / (16 / kC)) & (kC - 1); };
+    lds_t *const so = sbase + wave * kWaveOut;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int n = n0 + 16 * NB * wn + 16 * i + 4 * q4;
+        f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias && n < a.N) bias = *reinterpret_cast<const f32x4 *>(a.bias + n);
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+            const int r = 16 * j + l16;
+            const f32x4 v = acc[i][j] + bias;
+            *reinterpret_cast<__attribute__((address_space(3))) u32x2 *>(
+                so + r * (32 * NB) + (((2 * i + (q4 >> 1)) ^ swz(r)) << 4) + ((q4 & 1) << 3)) =
+                (u32x2){Elem<__bf16>::pack2(v.x, v.y), Elem<__bf16>::pack2(v.z, v.w)};
+        }
+    }
+    store_rows<16 * MB, kC>(a, so, swz, m0 + 16 * MB * wm, n0 + 16 * NB * wn, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -501,32 +746,37 @@ void f8_mm_tile(F8MmArgs a) {
                 (u32x2){Elem<__bf16>::pack2(v.x, v.y), Elem<__bf16>::pack2(v.z, v.w)};
         }
     }
-    typedef uint32_t u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));   // dst rows lie at multiples of 8 bytes
-    const int n = n0 + 128 * wn + 8 * l16;
-#pragma unroll
-    for (int t = 0; t < 32; ++t) {
-        const int r = 4 * t + q4, m = m0 + 128 * wm + r;
-        const u32x4 v = *reinterpret_cast<lds_u4 *>(so + r * 256 + ((l16 ^ (r & 15)) << 4));
-        char *const p = a.dst + (int64_t)m * a.d_nb1 + (int64_t)n * 2;
-        if (m < a.M) {
-            if (n + 8 <= a.N)
-                __builtin_nontemporal_store((u32x4_8)v, reinterpret_cast<u32x4_8 *>(p));
-            else if (n < a.N)
-                __builtin_nontemporal_store((u32x2){v.x, v.y}, reinterpret_cast<u32x2 *>(p));
-        }
-    }
+    store_rows<128, 16>(a, so, [](int r) { return r & 15; }, m0 + 128 * wm, n0 + 128 * wn, lane);
 }
 
-template <int NB, int MB, int D>
-static void launch_stream(const F8MmArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((f8_mm_stream<NB, MB, D>), dim3(a.n_blocks), dim3(256), 0, s, a);
+template <int NB, int MB, int S>
+static void launch_ring(const F8MmArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((f8_mm_ring<NB, MB, S>), dim3(a.n_blocks), dim3(256), 0, s, a);
+}
+
+template <int NB, int MB, int S>
+static void launch_grid(const F8MmArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((f8_mm_grid<NB, MB, S>), dim3(a.n_blocks), dim3(256), 0, s, a);
 }
 
 hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t s) {
     switch (tile) {
-    case 401: launch_stream<4, 1, 4>(a, s); break;
-    case 404: launch_stream<4, 4, 2>(a, s); break;
-    case 1616: hipLaunchKernelGGL(f8_mm_tile, dim3(a.n_blocks), dim3(256), 0, s, a); break;
+    case 101: launch_ring<1, 1, 4>(a, s); break;
+    case 201: launch_ring<2, 1, 4>(a, s); break;
+    case 401: launch_ring<4, 1, 3>(a, s); break;
+    case 202: launch_ring<2, 2, 4>(a, s); break;
+    case 402: launch_ring<4, 2, 3>(a, s); break;
+    case 404: launch_ring<4, 4, 2>(a, s); break;
+    case 405: launch_ring<4, 5, 1>(a, s); break;
+    case 804: launch_ring<8, 4, 1>(a, s); break;
+    case 805: launch_ring<8, 5, 1>(a, s); break;
+    case 10804: launch_grid<4, 2, 5>(a, s); break;
+    case 10806: launch_grid<4, 3, 5>(a, s); break;
+    case 10810: launch_grid<4, 5, 4>(a, s); break;
+    case 10812: launch_grid<4, 6, 3>(a, s); break;
+    case 10816: launch_grid<4, 8, 3>(a, s); break;
+    case 11608: launch_grid<8, 4, 3>(a, s); break;
+    case 11616: hipLaunchKernelGGL(f8_mm_tile, dim3(a.n_blocks), dim3(256), 0, s, a); break;
     default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

@@ -64,6 +64,9 @@ int check_f8(const kd_f8_rows &r, int64_t K) {
 // K values a row: whole 16-byte chunks of codes, 32-bit indexes
 int check_k(int64_t K) { return K <= 0 || K % 16 != 0 || K > kI32Max - 65536 ? KD_FA_ERR_SHAPE : KD_FA_OK; }
 
+// tiles of 16 * sixteens rows that cover `rows`
+int64_t tiles(int sixteens, int64_t rows) { return (rows + 16 * sixteens - 1) / (16 * sixteens); }
+
 size_t type_size(int type) {
     return type == KD_F8_TYPE_F32 ? 4 : type == KD_F8_TYPE_BF16 || type == KD_F8_TYPE_F16 ? 2 : 0;
 }
@@ -125,7 +128,7 @@ int validate(const kd_f8_mm_desc *d) {
     if (st != KD_FA_OK) return st;
     if (!same_rows(o, d->x.codes)) return KD_FA_ERR_SHAPE;
     const int64_t M = flat_rows(o);
-    if (M > kI32Max - 256) return KD_FA_ERR_SHAPE;
+    if (M > kI32Max - 256 || tiles(16, N) * tiles(16, M) > kdfa::kF8MmMaxBlocks) return KD_FA_ERR_SHAPE;
     // dst of no outputs has nothing to check but its width
     st = check_rows(o, N, 2, 8, N == 0 ? 0 : M);
     if (st != KD_FA_OK) return st;
@@ -135,7 +138,7 @@ int validate(const kd_f8_mm_desc *d) {
         if (st != KD_FA_OK) return st;
     }
     // a tile's rows are addressed with 32-bit offsets from its first
-    for (const kd_fa_tensor *t : {&d->w.codes, &d->w.scales, &d->x.codes, &d->x.scales, &o})
+    for (const kd_fa_tensor *t : {&d->w.codes, &d->w.scales, &d->x.codes, &d->x.scales})
         if (flat_rows(*t) > 1 && (uint64_t)t->nb[1] > kU32Max / 256) return KD_FA_ERR_LAYOUT;
     return KD_FA_OK;
 }
@@ -157,9 +160,31 @@ kdfa::F8RowsArgs rows_args(const kd_fa_tensor &x, const kd_f8_rows &out) {
 
 int launched(hipError_t e) { return e == hipSuccess ? KD_FA_OK : KD_FA_ERR_LAUNCH; }
 
+// The tile of a call: the one whose rounds of workgroups (256 CUs, `at_once`
+// on each) take least time.  A round's time with every CU at it is `fixed`
+// (first loads, sums and stores) + `stage` * the stages of 128 k; and the
+// rounds' stages take no less than the call's bytes from HBM (4.8 TB/s).  The
+// two figures of a tile are fitted to its times over 106 shapes (1 to 63,488
+// tokens, 4 to 16,384 outputs, 16 to 16,384 k); over these the tile taken is
+// in the mean 1.7% slower than the fastest of sixteen, at worst 21% (12,768 x
+// 1448 x 224, 31 us).  Six more tiles tried were never more than 1% of that
+// mean.
 int choose_tile(int64_t M, int64_t N, int64_t K) {
-    (void)N; (void)K;
-    return M <= 16 ? 401 : M < 64 ? 202 : M < 512 ? 405 : M < 3000 ? 10810 : 11616;
+    constexpr struct { int tile, at_once; double fixed, stage; } kTiles[] = {
+        {101, 2, 3.2, 0.067},   {202, 1, 3.2, 0.099},   {401, 1, 3.8, 0.072},   {402, 1, 3.9, 0.088},   {405, 1, 4.0, 0.20},
+        {10804, 1, 4.1, 0.22},  {10806, 1, 4.2, 0.29},  {10810, 1, 4.4, 0.455}, {10816, 1, 4.8, 0.68},  {11616, 1, 6.5, 1.14}};
+    const double stream = ((double)(M + N) * (double)K + 2.0 * (double)M * (double)N) / 4.8e6;   // us
+    const double stages = (double)blocks_of(K);
+    int best = 11616;
+    double least = 1e300;
+    for (const auto &t : kTiles) {
+        const int64_t n = tiles(t.tile / 100 % 100, N) * tiles(t.tile % 100, M);
+        if (t.tile != 11616 && n > kdfa::kF8MmMaxBlocks) continue;
+        const double rounds = (double)((n + 256 * t.at_once - 1) / (256 * t.at_once));
+        const double cost = rounds * t.fixed + std::max(rounds * t.stage * stages, stream);
+        if (cost < least) { least = cost; best = t.tile; }
+    }
+    return best;
 }
 
 }  // namespace
@@ -217,9 +242,7 @@ int kd_f8_mm_run(const kd_f8_mm_desc *desc, void *stream) {
     const int64_t K = desc->w.codes.ne[0], N = desc->w.codes.ne[1], M = flat_rows(desc->x.codes);
     if (M == 0 || N == 0) return KD_FA_OK;
     const int tile = choose_tile(M, N, K);
-    const int64_t tn = 16 * (tile / 100 % 100), tm = 16 * (tile % 100);
-    const int64_t tiles_n = (N + tn - 1) / tn, tiles_m = (M + tm - 1) / tm;
-    if (tiles_n * tiles_m > kdfa::kF8MmMaxBlocks) return KD_FA_ERR_SHAPE;
+    const int64_t tiles_n = tiles(tile / 100 % 100, N), tiles_m = tiles(tile % 100, M);
     st = kdfa::device_gfx950();
     if (st != KD_FA_OK) return st;
     kdfa::F8MmArgs a;

@@ -762,20 +762,14 @@ static void launch_grid(const F8MmArgs &a, hipStream_t s) {
 hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t s) {
     switch (tile) {
     case 101: launch_ring<1, 1, 4>(a, s); break;
-    case 201: launch_ring<2, 1, 4>(a, s); break;
-    case 401: launch_ring<4, 1, 3>(a, s); break;
     case 202: launch_ring<2, 2, 4>(a, s); break;
+    case 401: launch_ring<4, 1, 3>(a, s); break;
     case 402: launch_ring<4, 2, 3>(a, s); break;
-    case 404: launch_ring<4, 4, 2>(a, s); break;
     case 405: launch_ring<4, 5, 1>(a, s); break;
-    case 804: launch_ring<8, 4, 1>(a, s); break;
-    case 805: launch_ring<8, 5, 1>(a, s); break;
     case 10804: launch_grid<4, 2, 5>(a, s); break;
     case 10806: launch_grid<4, 3, 5>(a, s); break;
     case 10810: launch_grid<4, 5, 4>(a, s); break;
-    case 10812: launch_grid<4, 6, 3>(a, s); break;
     case 10816: launch_grid<4, 8, 3>(a, s); break;
-    case 11608: launch_grid<8, 4, 3>(a, s); break;
     case 11616: hipLaunchKernelGGL(f8_mm_tile, dim3(a.n_blocks), dim3(256), 0, s, a); break;
     default: return hipErrorInvalidValue;
     }

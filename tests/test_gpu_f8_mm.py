@@ -25,8 +25,21 @@ CASES = [
     (16, 68, 528, False), (16, 1000, 2064, True), (17, 64, 128, True), (31, 36, 640, False), (33, 100, 256, True), (47, 516, 1536, True),
     (64, 64, 512, False), (65, 68, 4112, True), (100, 1028, 272, True), (128, 128, 1024, False), (129, 132, 1040, True),
     (200, 260, 3600, True), (256, 256, 2048, False), (257, 516, 1168, True), (300, 4096, 128, True), (513, 772, 640, True),
-    (700, 1540, 912, False), (1280, 512, 256, True), (1999, 1024, 144, True), (4100, 300, 400, True),
+    (700, 1540, 912, False), (1280, 512, 256, True), (1999, 1024, 144, True), (4100, 300, 400, True), (434, 372, 608, True),
+    (97, 2164, 672, False), (34, 5576, 528, True), (290, 3816, 416, False), (1878, 788, 640, True), (3266, 856, 528, True),
+    (947, 3244, 784, False), (1531, 4720, 336, True), (2594, 6704, 192, True),
 ]
+# each tile's steady loop: many stages, the last whole or not
+DEEP = [
+    (3, 420, 5232, True), (17, 8, 6144, False), (18, 4104, 2240, True), (559, 444, 2048, False), (77, 2732, 3120, True),
+    (765, 260, 4096, False), (108, 2332, 4112, True), (1730, 136, 6144, True), (1556, 604, 2384, False), (1386, 544, 4096, True),
+    (176, 5716, 2384, True), (3695, 396, 3328, False), (1118, 1812, 4128, True), (4103, 412, 2304, False), (773, 4364, 6192, False),
+    (3461, 792, 2048, True), (1292, 3732, 2096, True), (1406, 4208, 4352, False), (1558, 6684, 2080, False), (3539, 2836, 4352, True),
+]
+# tokens and outputs that take the same tile for every K of STAGE_K: one to
+# thirteen stages, whole and not, through every kernel's first and last steps
+STAGES = [(1, 4), (46, 76), (27, 4880), (36, 4180), (238, 1128), (3000, 132), (888, 1616), (877, 2592), (3062, 1244), (5275, 1016), (3154, 3324)]
+STAGE_K = [16, 112, 128, 144, 256, 272, 384, 400, 512, 624, 640, 768, 784, 896, 1008, 1024, 1152, 1168, 1280, 1424, 1536, 1552, 1664]
 
 
 def _exact(M, N, K, bias, seed=0):
@@ -34,11 +47,17 @@ def _exact(M, N, K, bias, seed=0):
     xc, xs = exact_rows(rng, M, K)
     wc, ws = exact_rows(rng, N, K)
     b = rng.integers(-64, 65, N).astype(np.float32) if bias else None
-    want = of.linear(of.decode(xc, xs), of.decode(wc, ws), b)
+    # (float64 products of exact values, on the GPU where they are many)
+    xv, wv = (torch.from_numpy(of.decode(c, t)) for c, t in ((xc, xs), (wc, ws)))
+    if M * N * K > 1e9:
+        xv, wv = xv.to(DEV), wv.to(DEV)
+    want = (xv @ wv.t()).cpu().numpy()
+    if b is not None:
+        want = want + b.astype(np.float64)
     return (to_rows(xc, xs, DEV), to_rows(wc, ws, DEV), None if b is None else torch.from_numpy(b).to(DEV), round_bf16(want))
 
 
-@pytest.mark.parametrize("M,N,K,bias", CASES)
+@pytest.mark.parametrize("M,N,K,bias", CASES + DEEP)
 def test_exact_sums(M, N, K, bias):
     _need_gpu()
     announce(f"mm exact {M} x {N} x {K}")
@@ -50,6 +69,17 @@ def test_exact_sums(M, N, K, bias):
     assert torch.equal(store[1:M + 1, 4:4 + N].cpu(), want)
     store[1:M + 1, 4:4 + N] = 77.0
     assert bool((store == 77.0).all()), "written outside dst"
+
+
+@pytest.mark.parametrize("M,N", STAGES)
+def test_every_number_of_stages(M, N):
+    _need_gpu()
+    for K in STAGE_K:
+        announce(f"mm stages {M} x {N} x {K}")
+        x, w, b, want = _exact(M, N, K, True)
+        got = kd_f8.linear(x, w, b)
+        torch.cuda.synchronize()
+        assert torch.equal(got.cpu(), want), K
 
 
 @pytest.mark.parametrize("M,N,K,bias", [(2, 512, 4096, True), (16, 260, 3600, False), (60, 132, 992, True), (300, 516, 4096, True),

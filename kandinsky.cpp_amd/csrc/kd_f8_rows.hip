@@ -71,6 +71,21 @@ static __device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
     return x > o ? x : o;
 }
 
+// the sum over the 64 lanes, in every lane: of 16 by DPP, then by swaps of
+// rows of 16 and of 32 (a shuffle through LDS takes its latency each step)
+template <int CTRL>
+static __device__ __forceinline__ float add_dpp(float x) {
+    return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+static __device__ __forceinline__ float wave_sum(float x) {
+    x = add_dpp<0xb1>(x);    // lane ^ 1
+    x = add_dpp<0x4e>(x);    // lane ^ 2
+    x = add_dpp<0x141>(x);   // 7 - lane of each 8
+    x = add_dpp<0x140>(x);   // 15 - lane
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 // Eight values of a block (its 16 lanes call together) as codes; the block's
 // scale byte.  Magnitudes are compared as bits, where NaN is above infinity
 // and infinity above every number.  max|y| = f * 2^E with 1 <= f < 2: 2^e is
@@ -178,6 +193,17 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
             x[c].load(a.x + row * a.x_nb1, col < a.K ? col : 0);
             if constexpr (RES) r[c].load(a.residual + row * a.r_nb1, col < a.K ? col : 0);
         }
+        // the weights with them, where registers are plenty: few rows' latency
+        f32x4 w0[C], w1[C];
+        auto load_weight = [&](int c) __attribute__((always_inline)) {
+            const int col = 8 * (tid + T * c);
+            w0[c] = *reinterpret_cast<const f32x4 *>(a.weight + (col < a.K ? col : 0));
+            w1[c] = *reinterpret_cast<const f32x4 *>(a.weight + (col < a.K ? col : 0) + 4);
+        };
+        if constexpr (C <= 4) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) load_weight(c);
+        }
         float y[C][8];
         float ss = 0.0f;
 #pragma unroll
@@ -198,8 +224,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
                 ss += y[c][e] * y[c][e];
             }
         }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) ss += __shfl_xor(ss, m, 64);
+        ss = wave_sum(ss);
         if constexpr (kWaves > 1) {
             // two buffers in turn: a row's partial sums are read before the
             // next row's barrier, the row after that writes over them behind it
@@ -215,12 +240,11 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
         for (int c = 0; c < C; ++c) {
             const int col = 8 * (tid + T * c);
             const bool in = col < a.K;
-            const f32x4 w0 = *reinterpret_cast<const f32x4 *>(a.weight + (in ? col : 0));
-            const f32x4 w1 = *reinterpret_cast<const f32x4 *>(a.weight + (in ? col : 0) + 4);
+            if constexpr (C > 4) load_weight(c);
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float p = (y[c][e] * rstd) * (e < 4 ? w0[e] : w1[e - 4]);
+                const float p = (y[c][e] * rstd) * (e < 4 ? w0[c][e] : w1[c][e - 4]);
                 v[e] = in ? p : 0.0f;
             }
             uint32_t byte;

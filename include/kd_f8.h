@@ -106,7 +106,7 @@ typedef struct kd_f8_mm_desc {
 /*
  * Each *_supports returns 1 when its operator can execute the descriptor,
  * else 0 with the first failed condition's KD_FA_ERR_* code in *reason (when
- * reason != NULL).  Host-only.  K is at most 65536 for kd_f8_norm_run, whose
+ * reason != NULL).  Host-only.  K is at most 32768 for kd_f8_norm_run, whose
  * rows stay in registers.
  */
 int kd_f8_quantize_supports(const kd_f8_quantize_desc *desc, int *reason);

@@ -24,7 +24,7 @@ struct F8RowsArgs {
     float eps;
 };
 
-constexpr int kF8NormMaxK = 65536;
+constexpr int kF8NormMaxK = 32768;
 constexpr int kF8QuantBlocks = 64;   // blocks of 128 values per workgroup of quantize_kernel
 hipError_t launch_f8_quantize(const F8RowsArgs &a, hipStream_t stream);
 hipError_t launch_f8_norm(const F8RowsArgs &a, hipStream_t stream);

@@ -105,7 +105,7 @@ def test_norm_accepts(xt, rt):
     if xt == rt:
         kd_f8.norm_desc(x, w, rows(3, 5, 272), r, x)
     kd_f8.norm_desc(torch.zeros((0, 64), dtype=xt), torch.ones(64), rows(0, 64))
-    kd_f8.norm_desc(torch.zeros((1, 65536), dtype=xt), torch.ones(65536), rows(1, 65536), eps=0.0)
+    kd_f8.norm_desc(torch.zeros((1, 32768), dtype=xt), torch.ones(32768), rows(1, 32768), eps=0.0)
 
 
 def test_norm_refuses():
@@ -122,7 +122,7 @@ def test_norm_refuses():
     assert reason(lambda: kd_f8.norm_desc(x, w, out, torch.zeros((3, 32)), torch.zeros((3, 32)))) == kd_fa.ERR_SHAPE
     for eps in (-1e-6, float("nan"), float("inf")):
         assert reason(lambda: kd_f8.norm_desc(x, w, out, eps=eps)) == kd_fa.ERR_PARAM
-    big = 65536 + 16
+    big = 32768 + 16
     assert reason(lambda: kd_f8.norm_desc(torch.zeros((1, big)), torch.ones(big), rows(1, big))) == kd_fa.ERR_SHAPE
 
 

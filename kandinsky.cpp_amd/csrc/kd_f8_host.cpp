@@ -22,43 +22,50 @@ bool aligned(const void *p, uint64_t to) { return aligned((uint64_t)reinterpret_
 
 int64_t blocks_of(int64_t K) { return (K + kdfa::kF8Block - 1) / kdfa::kF8Block; }
 
-// rows of a [ne0, ne1, ne2, ne3] view, one stride apart; -1 on a layout that
-// has no one stride, or more rows than 32 bits count
-int64_t flat_rows(const kd_fa_tensor &t) {
-    if (t.ne[1] < 0 || t.ne[2] < 0 || t.ne[3] < 0) return -1;
-    if (t.ne[1] > kI32Max || t.ne[2] > kI32Max || t.ne[3] > kI32Max) return -1;
-    if (t.ne[1] == 0 || t.ne[2] == 0 || t.ne[3] == 0) return 0;
-    if (t.ne[2] > 1 && t.nb[2] != t.nb[1] * (size_t)t.ne[1]) return -1;
-    if (t.ne[3] > 1 && t.nb[3] != t.nb[2] * (size_t)t.ne[2]) return -1;
-    const int64_t two = t.ne[1] * t.ne[2];
-    if (two > kI32Max || two * t.ne[3] > kI32Max) return -1;
-    return two * t.ne[3];
+// The rows of a [ne0, ne1, ne2, ne3] view and the bytes from one to the next
+// (0 for a single row).  rows is -1 on a layout that has no one stride, or
+// more rows than 32 bits count.
+struct Rows { int64_t rows; uint64_t stride; };
+Rows flat_rows(const kd_fa_tensor &t) {
+    Rows r = {1, 0};
+    for (int i = 1; i < 4; ++i) {
+        if (t.ne[i] < 0) return {-1, 0};
+        if (t.ne[i] == 0) return {0, 0};
+    }
+    for (int i = 1; i < 4; ++i) {
+        if (t.ne[i] == 1) continue;
+        if (r.rows == 1) r.stride = t.nb[i];
+        else if (t.nb[i] != r.stride * (uint64_t)r.rows) return {-1, 0};
+        if (t.ne[i] > kI32Max / r.rows) return {-1, 0};
+        r.rows *= t.ne[i];
+    }
+    return r;
 }
 
 bool same_rows(const kd_fa_tensor &a, const kd_fa_tensor &b) {
     return a.ne[1] == b.ne[1] && a.ne[2] == b.ne[2] && a.ne[3] == b.ne[3];
 }
 
-// The row dimensions of every operand are x's (checked before); here: a view
-// of width `width`, elements of `size` bytes back to back, rows at multiples
-// of `align` that do not overlap.  `rows` is its number of rows.
-int check_rows(const kd_fa_tensor &t, int64_t width, size_t size, size_t align, int64_t rows) {
+// A view of width `width`, elements of `size` bytes back to back, rows at
+// multiples of `align` that do not overlap.
+int check_rows(const kd_fa_tensor &t, int64_t width, size_t size, size_t align) {
     if (t.ne[0] != width) return KD_FA_ERR_SHAPE;
-    if (rows < 0) return KD_FA_ERR_LAYOUT;
-    if (rows == 0) return KD_FA_OK;
+    const Rows r = flat_rows(t);
+    if (r.rows < 0) return KD_FA_ERR_LAYOUT;
+    if (r.rows == 0 || width == 0) return KD_FA_OK;
     if (!t.data) return KD_FA_ERR_NULL;
     if (t.nb[0] != size && width > 1) return KD_FA_ERR_LAYOUT;
     if (!aligned(t.data, align)) return KD_FA_ERR_LAYOUT;
-    if (rows > 1 && (!aligned(t.nb[1], align) || t.nb[1] < (uint64_t)width * size)) return KD_FA_ERR_LAYOUT;
+    if (r.rows > 1 && (!aligned(r.stride, align) || r.stride < (uint64_t)width * size)) return KD_FA_ERR_LAYOUT;
     return KD_FA_OK;
 }
 
 int check_f8(const kd_f8_rows &r, int64_t K) {
     if (r.codes.type != KD_F8_TYPE_E4M3 || r.scales.type != KD_F8_TYPE_E8M0) return KD_FA_ERR_TYPE;
     if (!same_rows(r.codes, r.scales)) return KD_FA_ERR_SHAPE;
-    const int st = check_rows(r.codes, K, 1, 16, flat_rows(r.codes));
+    const int st = check_rows(r.codes, K, 1, 16);
     if (st != KD_FA_OK) return st;
-    return check_rows(r.scales, blocks_of(K), 1, 4, flat_rows(r.scales));
+    return check_rows(r.scales, blocks_of(K), 1, 4);
 }
 
 // K values a row: whole 16-byte chunks of codes, 32-bit indexes
@@ -78,7 +85,7 @@ int validate(const kd_f8_quantize_desc *d) {
     int st = check_k(K);
     if (st != KD_FA_OK) return st;
     if (!same_rows(d->x, d->out.codes)) return KD_FA_ERR_SHAPE;
-    st = check_rows(d->x, K, type_size(d->x.type), 16, flat_rows(d->x));
+    st = check_rows(d->x, K, type_size(d->x.type), 16);
     return st != KD_FA_OK ? st : check_f8(d->out, K);
 }
 
@@ -91,22 +98,21 @@ int validate(const kd_f8_norm_desc *d) {
     if (st != KD_FA_OK) return st;
     if (K > kdfa::kF8NormMaxK) return KD_FA_ERR_SHAPE;
     if (!same_rows(d->x, d->out.codes)) return KD_FA_ERR_SHAPE;
-    const int64_t rows = flat_rows(d->x);
-    st = check_rows(d->x, K, type_size(d->x.type), 16, rows);
+    st = check_rows(d->x, K, type_size(d->x.type), 16);
     if (st != KD_FA_OK) return st;
     const kd_fa_tensor &r = d->residual, &s = d->sum, &w = d->weight;
-    if (rows > 0 && !r.data != !s.data) return KD_FA_ERR_NULL;
+    if (flat_rows(d->x).rows > 0 && !r.data != !s.data) return KD_FA_ERR_NULL;
     if (r.data) {
         if (!two_types(r.type) || s.type != r.type) return KD_FA_ERR_TYPE;
         if (!same_rows(d->x, r) || !same_rows(d->x, s)) return KD_FA_ERR_SHAPE;
-        st = check_rows(r, K, type_size(r.type), 16, flat_rows(r));
+        st = check_rows(r, K, type_size(r.type), 16);
         if (st != KD_FA_OK) return st;
-        st = check_rows(s, K, type_size(s.type), 16, flat_rows(s));
+        st = check_rows(s, K, type_size(s.type), 16);
         if (st != KD_FA_OK) return st;
     }
     if (w.type != KD_F8_TYPE_F32) return KD_FA_ERR_TYPE;
     if (w.ne[1] != 1 || w.ne[2] != 1 || w.ne[3] != 1) return KD_FA_ERR_SHAPE;
-    st = check_rows(w, K, 4, 16, 1);
+    st = check_rows(w, K, 4, 16);
     if (st != KD_FA_OK) return st;
     if (!std::isfinite(d->eps) || d->eps < 0.0f) return KD_FA_ERR_PARAM;
     return check_f8(d->out, K);
@@ -127,32 +133,33 @@ int validate(const kd_f8_mm_desc *d) {
     st = check_f8(d->x, K);
     if (st != KD_FA_OK) return st;
     if (!same_rows(o, d->x.codes)) return KD_FA_ERR_SHAPE;
-    const int64_t M = flat_rows(o);
+    const int64_t M = flat_rows(o).rows;
     if (M > kI32Max - 256 || tiles(16, N) * tiles(16, M) > kdfa::kF8MmMaxBlocks) return KD_FA_ERR_SHAPE;
-    // dst of no outputs has nothing to check but its width
-    st = check_rows(o, N, 2, 8, N == 0 ? 0 : M);
+    st = check_rows(o, N, 2, 8);
     if (st != KD_FA_OK) return st;
     if (b.data) {
         if (b.ne[1] != 1 || b.ne[2] != 1 || b.ne[3] != 1) return KD_FA_ERR_SHAPE;
-        st = check_rows(b, N, 4, 16, N == 0 ? 0 : 1);
+        st = check_rows(b, N, 4, 16);
         if (st != KD_FA_OK) return st;
     }
     // a tile's rows are addressed with 32-bit offsets from its first
     for (const kd_fa_tensor *t : {&d->w.codes, &d->w.scales, &d->x.codes, &d->x.scales})
-        if (flat_rows(*t) > 1 && (uint64_t)t->nb[1] > kU32Max / 256) return KD_FA_ERR_LAYOUT;
+        if (flat_rows(*t).stride > kU32Max / 256) return KD_FA_ERR_LAYOUT;
     return KD_FA_OK;
 }
+
+int64_t stride_of(const kd_fa_tensor &t) { return (int64_t)flat_rows(t).stride; }
 
 kdfa::F8RowsArgs rows_args(const kd_fa_tensor &x, const kd_f8_rows &out) {
     kdfa::F8RowsArgs a = {};
     a.x = static_cast<const char *>(x.data);
-    a.x_nb1 = (int64_t)x.nb[1];
+    a.x_nb1 = stride_of(x);
     a.x_type = x.type;
     a.codes = static_cast<char *>(out.codes.data);
-    a.c_nb1 = (int64_t)out.codes.nb[1];
+    a.c_nb1 = stride_of(out.codes);
     a.scales = static_cast<char *>(out.scales.data);
-    a.e_nb1 = (int64_t)out.scales.nb[1];
-    a.M = (int32_t)flat_rows(x);
+    a.e_nb1 = stride_of(out.scales);
+    a.M = (int32_t)flat_rows(x).rows;
     a.K = (int32_t)x.ne[0];
     a.blocks = (int32_t)blocks_of(x.ne[0]);
     return a;
@@ -225,9 +232,9 @@ int kd_f8_norm_run(const kd_f8_norm_desc *desc, void *stream) {
     kdfa::F8RowsArgs a = rows_args(desc->x, desc->out);
     if (a.M == 0) return KD_FA_OK;
     a.residual = static_cast<const char *>(desc->residual.data);
-    a.r_nb1 = (int64_t)desc->residual.nb[1];
+    a.r_nb1 = stride_of(desc->residual);
     a.sum = static_cast<char *>(desc->sum.data);
-    a.s_nb1 = (int64_t)desc->sum.nb[1];
+    a.s_nb1 = stride_of(desc->sum);
     a.s_type = desc->residual.type;
     a.weight = static_cast<const float *>(desc->weight.data);
     a.eps = desc->eps;
@@ -239,7 +246,7 @@ int kd_f8_norm_run(const kd_f8_norm_desc *desc, void *stream) {
 int kd_f8_mm_run(const kd_f8_mm_desc *desc, void *stream) {
     int st = validate(desc);
     if (st != KD_FA_OK) return st;
-    const int64_t K = desc->w.codes.ne[0], N = desc->w.codes.ne[1], M = flat_rows(desc->x.codes);
+    const int64_t K = desc->w.codes.ne[0], N = desc->w.codes.ne[1], M = flat_rows(desc->x.codes).rows;
     if (M == 0 || N == 0) return KD_FA_OK;
     const int tile = choose_tile(M, N, K);
     const int64_t tiles_n = tiles(tile / 100 % 100, N), tiles_m = tiles(tile % 100, M);
@@ -247,16 +254,16 @@ int kd_f8_mm_run(const kd_f8_mm_desc *desc, void *stream) {
     if (st != KD_FA_OK) return st;
     kdfa::F8MmArgs a;
     a.w = static_cast<const char *>(desc->w.codes.data);
-    a.w_nb1 = (int64_t)desc->w.codes.nb[1];
+    a.w_nb1 = stride_of(desc->w.codes);
     a.ws = static_cast<const char *>(desc->w.scales.data);
-    a.ws_nb1 = (int64_t)desc->w.scales.nb[1];
+    a.ws_nb1 = stride_of(desc->w.scales);
     a.x = static_cast<const char *>(desc->x.codes.data);
-    a.x_nb1 = (int64_t)desc->x.codes.nb[1];
+    a.x_nb1 = stride_of(desc->x.codes);
     a.xs = static_cast<const char *>(desc->x.scales.data);
-    a.xs_nb1 = (int64_t)desc->x.scales.nb[1];
+    a.xs_nb1 = stride_of(desc->x.scales);
     a.bias = static_cast<const float *>(desc->bias.data);
     a.dst = static_cast<char *>(desc->dst.data);
-    a.d_nb1 = M > 1 ? (int64_t)desc->dst.nb[1] : N * 2;   // (one row's stride may be anything)
+    a.d_nb1 = stride_of(desc->dst);
     a.M = (int32_t)M;
     a.N = (int32_t)N;
     a.K = (int32_t)K;

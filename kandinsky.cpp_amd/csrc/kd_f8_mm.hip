@@ -27,11 +27,18 @@ static __device__ __forceinline__ f32x4 mfma_f8(i32x8 a, i32x8 b, f32x4 c, uint3
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
 }
 
-// A DMA of one word per lane, each lane its own address, into 256 bytes of
-// LDS (as dma16: every consumer waits with an explicit s_waitcnt vmcnt).
-static __device__ __forceinline__ void dma4(const char *p, lds_t *lds_wave_base) {
+// DMAs into LDS, 16 bytes a lane at base + its offset, or one word a lane at
+// its own address; the destination is wave-uniform, the lanes' pieces lie there
+// in lane order.  The compiler does not track them: every consumer waits with
+// an explicit s_waitcnt vmcnt.  (m0 names the destination and takes a wait
+// state between its writing and the DMA.)
+static __device__ __forceinline__ void dma_16b(const char *base, uint32_t lane_off, lds_t *lds_wave_base) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_wave_base);
-    asm volatile("global_load_lds_dword %0, off" :: "v"(p), "{m0}"(m0));
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(lane_off), "s"(base), "{m0}"(m0));
+}
+static __device__ __forceinline__ void dma_word(const char *p, lds_t *lds_wave_base) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_wave_base);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(p), "{m0}"(m0));
 }
 
 static __device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
@@ -147,10 +154,10 @@ void f8_mm_ring(F8MmArgs a) {
             const int left = a.K - kt * 128;
             const uint32_t b0 = 16 * c0 < left ? 16 * c0 : 0, b1 = 16 * c1 < left ? 16 * c1 : 0;
 #pragma unroll
-            for (int j = 0; j < kDma; ++j) dma16((j < 2 * NB ? wt : xt) + kb, off[j] + (j & 1 ? b1 : b0), to + j * 1024);
+            for (int j = 0; j < kDma; ++j) dma_16b((j < 2 * NB ? wt : xt) + kb, off[j] + (j & 1 ? b1 : b0), to + j * 1024);
         } else {
 #pragma unroll
-            for (int j = 0; j < kDma; ++j) dma16(j < 2 * NB ? wt : xt, 0, to + j * 1024);
+            for (int j = 0; j < kDma; ++j) dma_16b(j < 2 * NB ? wt : xt, 0, to + j * 1024);
         }
     };
     // words first .. +count-1 of the tile's rows, [word][row]
@@ -161,7 +168,7 @@ void f8_mm_ring(F8MmArgs a) {
             const int r = 64 * h + lane, rx = r - 16 * NB;
             const bool w = rx < 0;
             const char *const p = w ? a.ws + (int64_t)(n0 + min(r, w_last)) * a.ws_nb1 : a.xs + (int64_t)(m0 + min(min(rx, 16 * MB - 1), x_last)) * a.xs_nb1;
-            for (int c = 0; c < count; ++c) dma4(p + 4 * (int64_t)(first + c), words + c * kWordRows * 4 + h * 256);
+            for (int c = 0; c < count; ++c) dma_word(p + 4 * (int64_t)(first + c), words + c * kWordRows * 4 + h * 256);
         }
     };
 
@@ -320,7 +327,7 @@ void f8_mm_grid(F8MmArgs a) {
             if (j == 0) {
                 const int g = min(kt >> 2, ng - 1);
 #pragma unroll
-                for (int h = 0; h < kWordDma; ++h) dma4(word_at[h] + 4 * (int64_t)g, words + ((kt >> 2) & 1) * kSlot + h * 1024 + wave * 256);
+                for (int h = 0; h < kWordDma; ++h) dma_word(word_at[h] + 4 * (int64_t)g, words + ((kt >> 2) & 1) * kSlot + h * 1024 + wave * 256);
             }
         }
         const char *at = (j < NB ? wt : xt) + (int64_t)kt * 128;
@@ -329,7 +336,7 @@ void f8_mm_grid(F8MmArgs a) {
             o = kt >= nk ? 0 : kt * 128 + 16 * dc < a.K ? o : off[j];
             at = kt >= nk ? (j < NB ? wt : xt) : at;
         }
-        dma16(at, o, sbase + buf * kStage + (wave + 4 * j) * 1024);
+        dma_16b(at, o, sbase + buf * kStage + (wave + 4 * j) * 1024);
     };
 
     f32x4 acc[NB][MB];
@@ -552,10 +559,10 @@ void f8_mm_tile(F8MmArgs a) {
         return t;
     };
     auto dma_w = [&](const Stage &t, int buf, int j) __attribute__((always_inline)) {
-        dma16(t.at, row_off(fresh(dr) + 32 * j, t.last, a.w_nb1) + t.chunk, sbase + buf * kTileBuf + (wave + 4 * j) * 1024);
+        dma_16b(t.at, row_off(fresh(dr) + 32 * j, t.last, a.w_nb1) + t.chunk, sbase + buf * kTileBuf + (wave + 4 * j) * 1024);
     };
     auto dma_x = [&](const Stage &t, int buf, int j) __attribute__((always_inline)) {
-        dma16(t.at, row_off(fresh(dr) + 32 * j, t.last, a.x_nb1) + t.chunk, sbase + (2 + buf) * kTileBuf + (wave + 4 * j) * 1024);
+        dma_16b(t.at, row_off(fresh(dr) + 32 * j, t.last, a.x_nb1) + t.chunk, sbase + (2 + buf) * kTileBuf + (wave + 4 * j) * 1024);
     };
 
     // scales: sw[i], sx[j] the words of row 16 i + l16 of this wave's halves.

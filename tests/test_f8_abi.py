@@ -64,6 +64,7 @@ def test_quantize_accepts(dt):
     kd_f8.quantize_desc(torch.zeros((0, 128), dtype=dt), rows(0, 128))
     kd_f8.quantize_desc(torch.zeros(128, dtype=dt), rows(128))
     kd_f8.quantize_desc(torch.zeros((4, 512), dtype=dt)[:, 128:384], rows(4, 256))     # strided rows
+    kd_f8.quantize_desc(torch.zeros((4, 7, 32), dtype=dt)[:, -1:], rows(4, 1, 32))     # each sequence's last row
 
 
 def test_quantize_refuses():

@@ -143,3 +143,22 @@ def test_an_explicit_stream_is_used():
     torch.cuda.synchronize()
     want, _ = of.quantize(np.full((1, 128), 50.0, dtype=np.float32))
     assert np.all(from_rows(r)[0] == want[0, 0])
+
+
+def test_last_token_of_each_sequence():
+    """Rows of a slice, one of each sequence, through every operator."""
+    _need_gpu()
+    announce("chain last tokens")
+    B, L, D = 5, 9, 512
+    blk = Block(D, 1024, 7)
+    g = torch.Generator().manual_seed(8)
+    branch = torch.randn((B, L, D), generator=g).to(BF16).to(DEV)
+    stream = torch.randn((B, L, D), generator=g).to(DEV)
+    got, total = blk(branch[:, -1:], stream[:, -1:])
+    want, same = blk(branch[:, -1].contiguous(), stream[:, -1].contiguous())
+    torch.cuda.synchronize()
+    assert got.shape == (B, 1, D) and torch.equal(got[:, 0], want) and torch.equal(total[:, 0], same)
+    whole, _ = kd_f8.add_rms_norm(branch, blk.norm, stream)
+    part = kd_f8.Rows(whole.codes[:, -1:], whole.scales[:, -1:])
+    assert torch.equal(kd_f8.linear(part, blk.up)[:, 0], kd_f8.linear(kd_f8.add_rms_norm(branch[:, -1].contiguous(), blk.norm,
+                                                                                         stream[:, -1].contiguous())[0], blk.up))

@@ -14,10 +14,10 @@ pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 # y = s * rstd * w in F32.  The sum of squares: each is rounded inside an FMA
-# or its addition, at most 64 in a lane, 6 steps over a wave and 16 waves: at
-# most 88 roundings of 2^-24 each, halved by the root; division, root and two
+# or its addition, at most 32 in a lane, 6 steps over a wave and 16 waves: at
+# most 54 roundings of 2^-24 each, halved by the root; division, root and two
 # products add 4 more.
-EPS_Y = 48 * 2.0 ** -24
+EPS_Y = 32 * 2.0 ** -24
 
 
 def _need_gpu():

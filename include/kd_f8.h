@@ -72,9 +72,10 @@ typedef struct kd_f8_quantize_desc {
 } kd_f8_quantize_desc;
 
 /*
- * kd_f8_norm_run: for each row, in F32,
- *   s = x + residual, rounded to sum's type (x itself without a residual)
- *   y = (s * (1 / sqrt(mean(s^2) + eps))) * weight
+ * kd_f8_norm_run: for each row
+ *   s = x + residual in F32, rounded to sum's type (x itself without one)
+ *   y = s / sqrt(mean(s^2) + eps) * weight, the mean summed in double and y
+ *       rounded to F32 (within 2^-23 of it)
  * sum = s, out = y in 8 bits.  residual and sum come together: both given or
  * neither (data == NULL).
  */

@@ -74,16 +74,22 @@ static __device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
 // the sum over the 64 lanes, in every lane: of 16 by DPP, then by swaps of
 // rows of 16 and of 32 (a shuffle through LDS takes its latency each step)
 template <int CTRL>
-static __device__ __forceinline__ float add_dpp(float x) {
-    return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+static __device__ __forceinline__ double add_dpp(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return x + __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
-static __device__ __forceinline__ float wave_sum(float x) {
+static __device__ __forceinline__ double wave_sum(double x) {
     x = add_dpp<0xb1>(x);    // lane ^ 1
     x = add_dpp<0x4e>(x);    // lane ^ 2
     x = add_dpp<0x141>(x);   // 7 - lane of each 8
     x = add_dpp<0x140>(x);   // 15 - lane
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+    return pair_sum_f64(__builtin_bit_cast(double, (uint64_t)lo[0] | ((uint64_t)hi[0] << 32)) +
+                        __builtin_bit_cast(double, (uint64_t)lo[1] | ((uint64_t)hi[1] << 32)));
 }
 
 // Eight values of a block (its 16 lanes call together) as codes; the block's
@@ -177,12 +183,15 @@ __global__ __launch_bounds__(256) void quantize_kernel(F8RowsArgs a) {
 // in registers between its one reading and its writing.  Bound by HBM for
 // many rows (63,488 x 4096, BF16 onto an F32 stream, 2.86 GB: 0.52 ms, 5.5
 // TB/s, what a copy reaches), by one row's latency for few (2 x 3584: 2.8 us).
+// A code is a rounding to 4 bits, and a value next to its border goes to the
+// wrong side by an error of the value's last bits: so the squares are summed in
+// double and each value of the norm is rounded once (both under the loads).
 // ---------------------------------------------------------------------------
 template <int XT, int ST, bool RES, int T, int C>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
     constexpr int kRows = T < 256 ? 256 / T : 1;   // rows at once in a workgroup
     constexpr int kWaves = T / 64;
-    __shared__ float part[2][kWaves];
+    __shared__ double part[2][kWaves];
     const int tid = threadIdx.x % T;
     const int lane = threadIdx.x & 63;
     int turn = 0;
@@ -207,7 +216,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
             for (int c = 0; c < C; ++c) load_weight(c);
         }
         float y[C][8];
-        float ss = 0.0f;
+        double ss = 0.0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = 8 * (tid + T * c);
@@ -223,7 +232,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 y[c][e] = in ? y[c][e] : 0.0f;
-                ss += y[c][e] * y[c][e];
+                ss += (double)y[c][e] * (double)y[c][e];
             }
         }
         ss = wave_sum(ss);
@@ -232,12 +241,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
             // next row's barrier, the row after that writes over them behind it
             if (lane == 0) part[turn][tid >> 6] = ss;
             __syncthreads();
-            ss = 0.0f;
+            ss = 0.0;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) ss += part[turn][w];
             turn ^= 1;
         }
-        const float rstd = 1.0f / sqrt_rn(ss / (float)a.K + a.eps);
+        // 1 / rms as the sum of two F32
+        const double rstd = 1.0 / __builtin_sqrt(ss / (double)a.K + (double)a.eps);
+        const float r0 = (float)rstd, r1 = (float)(rstd - (double)r0);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = 8 * (tid + T * c);
@@ -246,8 +257,11 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float p = (y[c][e] * rstd) * (e < 4 ? w0[c][e] : w1[c][e - 4]);
-                v[e] = in ? p : 0.0f;
+                // y / rms * weight, rounded once: the product with what its
+                // rounding left
+                const float w = e < 4 ? w0[c][e] : w1[c][e - 4], p = y[c][e] * r0;
+                const float q = __builtin_fmaf(y[c][e], r1, __builtin_fmaf(y[c][e], r0, -p));
+                v[e] = in ? __builtin_fmaf(p, w, q * w) : 0.0f;
             }
             uint32_t byte;
             const u32x2 q = to_f8(v, byte);

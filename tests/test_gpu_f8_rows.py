@@ -13,11 +13,11 @@ from f8_common import DEV, announce, from_rows
 pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
-# y = s * rstd * w in F32.  The sum of squares: each is rounded inside an FMA
-# or its addition, at most 32 in a lane, 6 steps over a wave and 16 waves: at
-# most 54 roundings of 2^-24 each, halved by the root; division, root and two
-# products add 4 more.
-EPS_Y = 32 * 2.0 ** -24
+# y = s / rms * w.  rms is within a few roundings of double; as two F32 it is
+# within 2^-48.  s / rms is a product and what its rounding left, the latter
+# within 2^-24 of itself twice over: 2^-46 of the product; times w that rest is
+# rounded again, 2^-48, and the sum once, 2^-24.  In all less than 2^-23.
+EPS_Y = 2.0 ** -23
 
 
 def _need_gpu():

@@ -51,6 +51,7 @@ def test_rows_hold_codes_and_their_scales():
     assert r.codes.shape == (2, 3, 272) and r.scales.shape == (2, 3, 3) and r.scales.stride() == (12, 4, 1)
     r.scales.view(torch.uint8).fill_(127)
     assert torch.equal(r.to("cpu").scales.view(torch.uint8), r.scales.view(torch.uint8))
+    assert rows(3, 1040).codes.stride() == (1152, 1) and rows(3, 1040).codes.shape == (3, 1040)
     with pytest.raises(ValueError):
         kd_f8.Rows(torch.zeros((4, 128)), r.scales)
     with pytest.raises(ValueError):

@@ -134,7 +134,7 @@ int validate(const kd_f8_mm_desc *d) {
     if (st != KD_FA_OK) return st;
     if (!same_rows(o, d->x.codes)) return KD_FA_ERR_SHAPE;
     const int64_t M = flat_rows(o).rows;
-    if (M > kI32Max - 256 || tiles(16, N) * tiles(16, M) > kdfa::kF8MmMaxBlocks) return KD_FA_ERR_SHAPE;
+    if (M > kI32Max - 256 || tiles(8, N) * tiles(16, M) > kdfa::kF8MmMaxBlocks) return KD_FA_ERR_SHAPE;
     st = check_rows(o, N, 2, 8);
     if (st != KD_FA_OK) return st;
     if (b.data) {
@@ -182,11 +182,11 @@ int choose_tile(int64_t M, int64_t N, int64_t K) {
         {10804, 1, 4.1, 0.22},  {10806, 1, 4.2, 0.29},  {10810, 1, 4.4, 0.455}, {10816, 1, 4.8, 0.68},  {11616, 1, 6.5, 1.14}};
     const double stream = ((double)(M + N) * (double)K + 2.0 * (double)M * (double)N) / 4.8e6;   // us
     const double stages = (double)blocks_of(K);
-    int best = 11616;
+    int best = 10816;   // (the largest that takes any size)
     double least = 1e300;
     for (const auto &t : kTiles) {
         const int64_t n = tiles(t.tile / 100 % 100, N) * tiles(t.tile % 100, M);
-        if (t.tile != 11616 && n > kdfa::kF8MmMaxBlocks) continue;
+        if (n > kdfa::kF8MmMaxBlocks || (t.tile == 11616 && (M < 256 || N < 256))) continue;
         const double rounds = (double)((n + 256 * t.at_once - 1) / (256 * t.at_once));
         const double cost = rounds * t.fixed + std::max(rounds * t.stage * stages, stream);
         if (cost < least) { least = cost; best = t.tile; }

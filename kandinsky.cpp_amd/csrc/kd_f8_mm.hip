@@ -491,10 +491,11 @@ void f8_mm_grid(F8MmArgs a) {
 //
 // A row's scales come as words of four stages, loaded by the lanes that hold
 // the row, a step ahead of their first use.
-// Rows past M or N are the last row again (not stored).  The last steps bring
-// nothing past K: a stage that is not there is the tile's first chunk for
-// every lane, a chunk past K its row's first of that stage, and X's are
-// zeroed in their registers.
+// M and N are at least 256: a last tile that would end past them begins earlier
+// instead, and what it has in common with the one before is written twice, the
+// same bits.  The last steps bring nothing past K: a stage that is not there is
+// the tile's first chunk for every lane, a chunk past K its row's first of that
+// stage, and X's are zeroed in their registers.
 // ---------------------------------------------------------------------------
 constexpr int kTileBuf = 32768;   // 256 rows x 128 k
 
@@ -522,47 +523,42 @@ void f8_mm_tile(F8MmArgs a) {
     const int wn = wave & 1, wm = wave >> 1;
     int nt, mt;
     f8_tile(a, nt, mt);
-    const int n0 = nt * 256, m0 = mt * 256;
+    const int n0 = min(nt * 256, a.N - 256), m0 = min(mt * 256, a.M - 256);
     const int nk = (int)(((uint32_t)a.K + 127) >> 7);   // stages
     const int whole = a.K >> 7;                         // those of 128 k
     const int ng = (nk + 3) >> 2;                       // words of scales
 
-    // DMA j of a wave: rows 8 (wave + 4 j) .. +7, lane l the chunk that lies
-    // at l % 8 of row l / 8.  Row offsets are made where they are used (a few
-    // instructions under a product), not kept in registers: `fresh` hides from
-    // the compiler that they are the same every time.
-    const int dr = 8 * wave + (lane >> 3);
-    const int dc = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
-    const int w_last = a.N - 1 - n0, x_last = a.M - 1 - m0;
-    auto fresh = [](int v) __attribute__((always_inline)) {
-        asm volatile("" : "+v"(v));
-        return v;
-    };
-    auto row_off = [](int r, int last, int64_t nb1) __attribute__((always_inline)) {
-        return __umul24((uint32_t)min(r, last), (uint32_t)nb1);   // (strides are below 2^24: kd_f8_host.cpp)
-    };
     const char *const wtile = a.w + (int64_t)n0 * a.w_nb1;
     const char *const xtile = a.x + (int64_t)m0 * a.x_nb1;
     const char *const wst = a.ws + (int64_t)n0 * a.ws_nb1;
     const char *const xst = a.xs + (int64_t)m0 * a.xs_nb1;
-    // Stage kt of W or X: its first byte of the tile's first row, the tile's
-    // last row and the lane's chunk.  A stage that is not there is the tile's
-    // first chunk for every lane, a chunk past K its row's first.
-    struct Stage { const char *at; int last; uint32_t chunk; };
-    auto stage = [&](const char *tile, int last, int kt, auto end_c) __attribute__((always_inline)) {
-        Stage t = {tile + (int64_t)kt * 128, last, (uint32_t)(dc << 4)};
+    // DMA j of a wave: rows 8 (wave + 4 j) .. +7, lane l the chunk that lies
+    // at l % 8 of row l / 8: one offset a lane, and a scalar step from j to j
+    // + 1.  (Offsets clamped to the last row were four vector instructions a
+    // DMA, as many as products: 903 us, without them 873, at 63,488 x 4096 x
+    // 4096.)
+    const int dr = 8 * wave + (lane >> 3);
+    const int dc = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+    const uint32_t w_row = __umul24(dr, (uint32_t)a.w_nb1), x_row = __umul24(dr, (uint32_t)a.x_nb1);   // (strides are below 2^24)
+    const uint32_t w_off = w_row + (dc << 4), x_off = x_row + (dc << 4);
+    // Stage kt of W or X.  One that is not there is the tile's first chunk for
+    // every lane, a chunk past K its row's first.
+    struct Stage { const char *at; int64_t step; uint32_t off; };
+    auto stage = [&](bool w, int kt, auto end_c) __attribute__((always_inline)) {
+        const char *const tile = w ? wtile : xtile;
+        Stage t = {tile + (int64_t)kt * 128, 32 * (w ? a.w_nb1 : a.x_nb1), w ? w_off : x_off};
         if constexpr (decltype(end_c)::value) {
-            t.chunk = kt * 128 + 16 * dc < a.K ? t.chunk : 0;
-            t.last = kt < nk ? last : 0;
+            t.off = kt * 128 + 16 * dc < a.K ? t.off : kt < nk ? (w ? w_row : x_row) : 0;
             t.at = kt < nk ? t.at : tile;
+            t.step = kt < nk ? t.step : 0;
         }
         return t;
     };
     auto dma_w = [&](const Stage &t, int buf, int j) __attribute__((always_inline)) {
-        dma_16b(t.at, row_off(fresh(dr) + 32 * j, t.last, a.w_nb1) + t.chunk, sbase + buf * kTileBuf + (wave + 4 * j) * 1024);
+        dma_16b(t.at + j * t.step, t.off, sbase + buf * kTileBuf + (wave + 4 * j) * 1024);
     };
     auto dma_x = [&](const Stage &t, int buf, int j) __attribute__((always_inline)) {
-        dma_16b(t.at, row_off(fresh(dr) + 32 * j, t.last, a.x_nb1) + t.chunk, sbase + (2 + buf) * kTileBuf + (wave + 4 * j) * 1024);
+        dma_16b(t.at + j * t.step, t.off, sbase + (2 + buf) * kTileBuf + (wave + 4 * j) * 1024);
     };
 
     // scales: sw[i], sx[j] the words of row 16 i + l16 of this wave's halves.
@@ -577,7 +573,7 @@ void f8_mm_tile(F8MmArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const bool w = q < 2;
-            const uint32_t r = row_off(fresh(lane) + (w ? 128 * wn : 128 * wm) + 64 * (q & 1), w ? w_last : x_last, w ? a.ws_nb1 : a.xs_nb1);
+            const uint32_t r = __umul24(lane + (w ? 128 * wn : 128 * wm) + 64 * (q & 1), (uint32_t)(w ? a.ws_nb1 : a.xs_nb1));
             const char *const row = (w ? wst : xst) + (uint64_t)r;
             if (4 * b + 4 <= ng) {
                 raw[q] = *reinterpret_cast<const u32x4_4 *>(row + 16 * b);
@@ -626,7 +622,7 @@ void f8_mm_tile(F8MmArgs a) {
         constexpr int S = decltype(sel_c)::value, P = S & 1;
         constexpr bool END = decltype(end_c)::value;
         const int xprev = xb == 0 ? 2 : xb - 1;   // freed by the last step's barrier
-        const Stage next_w = stage(wtile, w_last, kt + 2, end_c), next_x = stage(xtile, x_last, kt + 3, end_c);
+        const Stage next_w = stage(true, kt + 2, end_c), next_x = stage(false, kt + 3, end_c);
         if constexpr (END) {
             if (kt >= whole) {
                 // the one stage that ends inside: what lies past K is zero
@@ -682,9 +678,8 @@ void f8_mm_tile(F8MmArgs a) {
 
     load_scales(0);
     {
-        const Stage x0 = stage(xtile, x_last, 0, BC<true>()), w0 = stage(wtile, w_last, 0, BC<true>()),
-                    x1 = stage(xtile, x_last, 1, BC<true>()), w1 = stage(wtile, w_last, 1, BC<true>()),
-                    x2 = stage(xtile, x_last, 2, BC<true>());
+        const Stage x0 = stage(false, 0, BC<true>()), w0 = stage(true, 0, BC<true>()), x1 = stage(false, 1, BC<true>()),
+                    w1 = stage(true, 1, BC<true>()), x2 = stage(false, 2, BC<true>());
 #pragma unroll
         for (int j = 0; j < 8; ++j) dma_x(x0, 0, j);
 #pragma unroll
@@ -744,7 +739,7 @@ void f8_mm_tile(F8MmArgs a) {
     for (int i = 0; i < 8; ++i) {
         const int n = n0 + 128 * wn + 16 * i + 4 * q4;
         f32x4 bias = {0.f, 0.f, 0.f, 0.f};
-        if (a.bias && n < a.N) bias = *reinterpret_cast<const f32x4 *>(a.bias + n);
+        if (a.bias) bias = *reinterpret_cast<const f32x4 *>(a.bias + n);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const f32x4 v = acc[i][j] + bias;

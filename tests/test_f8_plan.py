@@ -10,7 +10,7 @@ from f8_plan import TILES, desc, outputs, plan, run, tokens
 from test_gpu_f8_mm import CASES, DEEP, STAGE_K, STAGES
 
 
-@pytest.mark.parametrize("M,N,K", [(2 ** 31 - 257, 4, 32), (1, 2 ** 31 - 260, 32), (200, 2 ** 31 - 512, 64), (2 ** 24, 2 ** 14, 16),
+@pytest.mark.parametrize("M,N,K", [(2 ** 31 - 257, 4, 32), (1, 2 ** 30 - 4, 32), (200, 2 ** 30 - 512, 64), (2 ** 24, 2 ** 14, 16),
                                    (1, 4, 2 ** 31 - 65536 - 16 - (2 ** 31 - 65536) % 16)])
 def test_sizes_within_a_tile_of_2_31(M, N, K):
     d = desc(M, N, K)
@@ -30,8 +30,9 @@ def test_sizes_within_a_tile_of_2_31(M, N, K):
 
 
 def test_more_tiles_than_a_launch_holds_are_refused():
-    st, _ = run(desc(2 ** 26, 2 ** 21, 16))
-    assert st == kd_fa.ERR_SHAPE
+    for M, N in ((2 ** 26, 2 ** 21), (1, 2 ** 31 - 260), (257, 2 ** 30)):
+        st, _ = run(desc(M, N, 32))
+        assert st == kd_fa.ERR_SHAPE
 
 
 def test_one_row_of_dst_may_have_any_stride():
@@ -49,6 +50,7 @@ def test_every_size_has_a_tile_and_it_covers_the_call():
         p = plan(M, N // 4 * 4, K // 16 * 16)
         seen.add(p.tile)
         assert p.n_blocks == -(-p.M // tokens(p.tile)) * -(-p.N // outputs(p.tile))
+        assert p.tile != 11616 or (M >= 256 and N >= 256)      # its tiles are whole
     assert seen == set(TILES)      # none that no call reaches
 
 

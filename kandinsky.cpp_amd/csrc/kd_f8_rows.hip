@@ -246,9 +246,21 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
             for (int w = 0; w < kWaves; ++w) ss += part[turn][w];
             turn ^= 1;
         }
-        // 1 / rms as the sum of two F32
-        const double rstd = 1.0 / __builtin_sqrt(ss / (double)a.K + (double)a.eps);
-        const float r0 = (float)rstd, r1 = (float)(rstd - (double)r0);
+        // 1 / rms as the sum of two F32; of rows so small or large that these
+        // would not be normal numbers, 2^100 goes over to y (exact, but for
+        // what is nothing beside the row's largest)
+        double rstd = 1.0 / __builtin_sqrt(ss / (double)a.K + (double)a.eps);
+        if (!(rstd >= 0x1p-100 && rstd <= 0x1p100)) {
+            const float up = rstd > 1.0 ? 0x1p100f : 0x1p-100f;
+            rstd *= rstd > 1.0 ? 0x1p-100 : 0x1p100;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[c][e] *= up;
+        }
+        float r0 = (float)rstd;
+        if ((double)r0 > rstd) r0 = __uint_as_float(__float_as_uint(r0) - 1);   // (r1 >= 0)
+        const float r1 = (float)(rstd - (double)r0);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int col = 8 * (tid + T * c);
@@ -258,9 +270,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 // y / rms * weight, rounded once: the product with what its
-                // rounding left
+                // rounding left (a zero with the product's sign, so that -0
+                // stays what it is)
                 const float w = e < 4 ? w0[c][e] : w1[c][e - 4], p = y[c][e] * r0;
-                const float q = __builtin_fmaf(y[c][e], r1, __builtin_fmaf(y[c][e], r0, -p));
+                const float q = __builtin_fmaf(y[c][e], r1, -__builtin_fmaf(-y[c][e], r0, p));
                 v[e] = in ? __builtin_fmaf(p, w, q * w) : 0.0f;
             }
             uint32_t byte;

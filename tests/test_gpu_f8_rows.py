@@ -14,9 +14,9 @@ pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 # y = s / rms * w.  rms is within a few roundings of double; as two F32 it is
-# within 2^-48.  s / rms is a product and what its rounding left, the latter
+# within 2^-47.  s / rms is a product and what its rounding left, the latter
 # within 2^-24 of itself twice over: 2^-46 of the product; times w that rest is
-# rounded again, 2^-48, and the sum once, 2^-24.  In all less than 2^-23.
+# rounded again, 2^-47, and the sum once, 2^-24.  In all less than 2^-23.
 EPS_Y = 2.0 ** -23
 
 
@@ -219,6 +219,24 @@ def test_norm_without_eps_and_with_a_large_one():
         out, _ = kd_f8.add_rms_norm(x, w, eps=eps)
         torch.cuda.synchronize()
         check_norm(x, None, w, eps, out, None)
+
+
+@pytest.mark.parametrize("K", [256, 3600, 16400])
+def test_norm_of_rows_at_either_end_of_f32(K):
+    """Without eps: 1 / rms beyond F32, below its normal numbers, and near."""
+    _need_gpu()
+    announce(f"norm ends of F32, {K}")
+    x = torch.randn((9, K), generator=torch.Generator().manual_seed(11)).clamp(-4, 4)
+    for i, top in enumerate((1e-44, 1e-40, 1e-38, 2.0 ** -99, 2.0 ** 99, 1e37, 8e37)):
+        x[i] *= top
+    x[7] = 0.0
+    x[7, K - 1] = 1e-45
+    x[8] = float(np.finfo(np.float32).max)
+    w = 1 + 0.3 * torch.rand(K, generator=torch.Generator().manual_seed(12))
+    for r in (None, torch.zeros_like(x)):
+        out, total = kd_f8.add_rms_norm(x.to(DEV), w.to(DEV), None if r is None else r.to(DEV), eps=0.0)
+        torch.cuda.synchronize()
+        check_norm(x, r, w, 0.0, out, total)
 
 
 def test_norm_of_more_rows_than_workgroups():

@@ -10,11 +10,12 @@ bytes (`empty_rows` makes them so, and lays the codes out as the product
 reads them fastest).  Each operator has a descriptor over
 existing tensors (`quantize_desc`, `norm_desc`, `linear_desc`), checked when
 it is made, which `run` launches any number of times; the functions above
-make their outputs and run once.  Inference only: no gradient is recorded.
+make their outputs -- tensors of the stream they run on -- and run once.  Inference only: no gradient is recorded.
 There is no fallback path: the library must be built.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -203,9 +204,16 @@ def _current_stream(dev) -> int:
     return raw(dev.index) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
+def _made_on(stream):
+    """Tensors made in this context belong to `stream`: on another stream
+    their memory might still be in use by what was enqueued there."""
+    return contextlib.nullcontext() if stream is None else kd_fa._torch().cuda.stream(stream)
+
+
 def quantize(x, stream=None) -> Rows:
     """x (..., K) as 8-bit rows."""
-    out = empty_rows(x.shape[:-1], x.shape[-1], x.device)
+    with _made_on(stream):
+        out = empty_rows(x.shape[:-1], x.shape[-1], x.device)
     run(quantize_desc(x, out), stream)
     return out
 
@@ -214,8 +222,9 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6, stream=None):
     """(Rows, sum): the RMS norm of x + residual in 8 bits, and the addition
     in residual's type -- (Rows, x) without a residual."""
     torch = kd_fa._torch()
-    out = empty_rows(x.shape[:-1], x.shape[-1], x.device)
-    total = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+    with _made_on(stream):
+        out = empty_rows(x.shape[:-1], x.shape[-1], x.device)
+        total = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)
     run(norm_desc(x, weight, out, residual, total, eps), stream)
     return out, x if total is None else total
 
@@ -224,6 +233,7 @@ def linear(x: Rows, w: Rows, bias=None, dst=None, stream=None):
     """ops::linear on 8-bit rows: x (..., K) and w (N, K) -> (..., N) bfloat16."""
     torch = kd_fa._torch()
     if dst is None:
-        dst = torch.empty(tuple(x.shape[:-1]) + (w.shape[0],), dtype=torch.bfloat16, device=x.codes.device)
+        with _made_on(stream):
+            dst = torch.empty(tuple(x.shape[:-1]) + (w.shape[0],), dtype=torch.bfloat16, device=x.codes.device)
     run(linear_desc(x, w, dst, bias), stream)
     return dst

@@ -145,6 +145,38 @@ def test_an_explicit_stream_is_used():
     assert np.all(from_rows(r)[0] == want[0, 0])
 
 
+def test_outputs_of_an_explicit_stream_are_its_own():
+    """What the current stream still writes to, and has given back, is not
+    handed to a call on another stream."""
+    _need_gpu()
+    announce("chain explicit stream's outputs")
+    s = torch.cuda.Stream()
+    x = torch.full((4096, 4096), 50.0, device=DEV)
+    w = kd_f8.quantize(torch.eye(4096, device=DEV))
+    codes, scales = from_rows(kd_f8.quantize(x))
+    torch.cuda.synchronize()
+
+    def busy(shape, dtype):
+        old = torch.empty(shape, dtype=dtype, device=DEV)
+        for _ in range(200):
+            old.fill_(7)
+
+    busy((4096, 4096), torch.uint8)
+    r = kd_f8.quantize(x, stream=s)
+    torch.cuda.synchronize()
+    assert np.array_equal(from_rows(r)[0], codes) and np.array_equal(from_rows(r)[1], scales)
+    busy((4096, 4096), torch.bfloat16)
+    y = kd_f8.linear(r, w, stream=s)
+    torch.cuda.synchronize()
+    # 50 lies halfway between two codes: blocks of 50s get the scale 2^-3, 400
+    # = 1.5625 * 2^8 goes to 1.5 * 2^8 (of 1.5 and 1.625 the even one)
+    assert bool((y == 48.0).all())
+    busy((4096, 4096), torch.float32)
+    _, total = kd_f8.add_rms_norm(x, torch.ones(4096, device=DEV), x, stream=s)
+    torch.cuda.synchronize()
+    assert bool((total == 100.0).all())
+
+
 def test_last_token_of_each_sequence():
     """Rows of a slice, one of each sequence, through every operator."""
     _need_gpu()

@@ -238,6 +238,7 @@ int kd_f8_norm_run(const kd_f8_norm_desc *desc, void *stream) {
     a.s_type = desc->residual.type;
     a.weight = static_cast<const float *>(desc->weight.data);
     a.eps = desc->eps;
+    a.inv_k = 1.0 / a.K;
     st = kdfa::device_gfx950();
     if (st != KD_FA_OK) return st;
     return launched(kdfa::launch_f8_norm(a, static_cast<hipStream_t>(stream)));

@@ -22,6 +22,7 @@ struct F8RowsArgs {
     int32_t x_type, s_type; // KD_F8_TYPE_* of x; of residual and sum
     int32_t M, K, blocks;
     float eps;
+    double inv_k;           // norm: 1 / K
 };
 
 constexpr int kF8NormMaxK = 32768;

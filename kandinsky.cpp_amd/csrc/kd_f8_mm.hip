@@ -102,6 +102,12 @@ static __device__ __forceinline__ void store_rows(const F8MmArgs &a, const lds_t
 // In LDS 16-byte chunk c of row r lies at c ^ ((r >> 1) & 7).  Rows past N or
 // M are the last row again (not stored); a chunk past K is its row's first of
 // the stage, X's then zeroed in the registers.
+//
+// With few tokens it is bound by W's way from HBM: 2 x 16384 x 4096 (67 MB)
+// 12.3 us, 5.5 TB/s, what a copy reaches.  300 x 4096 x 4096 takes 12.5 us
+// (256 tiles of 64 x 80, one on each CU): 4 of it the first loads, the sums and
+// the stores, and 0.2 for each of the 32 stages, whose 18 KB then come into LDS
+// at 23 TB/s over all CUs, out of the L2s.
 // ---------------------------------------------------------------------------
 constexpr int kRingWords = 8;   // words of scales per row at a time
 
@@ -272,6 +278,12 @@ void f8_mm_ring(F8MmArgs a) {
 // each fourth stage, into one of two slots.  LDS rows, rows past N or M and k
 // past K are f8_mm_ring's; a stage past the last is the tile's first chunk for
 // every lane, so that the counter counts alike.
+//
+// 1,280 x 4096 x 4096 takes 23.5 us (256 tiles of 128 x 160, one on each CU):
+// 0.46 us a stage for the CU's 36 KB into LDS, 20 TB/s over all of them out of
+// the L2s, where the products would take 0.31 at the rate they sustain.  997 x
+// 1540 x 3600: 17.8 us (208 tiles of 128 x 64), 13.1 with the rows padded to
+// whole lines.
 // ---------------------------------------------------------------------------
 template <int NB, int MB, int S>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
@@ -491,6 +503,15 @@ void f8_mm_grid(F8MmArgs a) {
 //
 // A row's scales come as words of four stages, loaded by the lanes that hold
 // the row, a step ahead of their first use.
+//
+// 63,488 x 4096 x 4096 takes 0.86-0.87 ms (2.45 PFLOP/s), 15,872 x 4096 x 16384
+// 0.74 (2.88); the products alone (no loads, no LDS reads) would take 0.50 of
+// the former, the DMAs alone 0.53-0.62.  Both together draw the chip down to
+// 2.0-2.1 GHz, and the two run at once but for what the barrier holds up.
+// Tiles kept up by persistent workgroups (the next tile's first stages under
+// the stores), lines asked into the L2 ahead, other cache hints of the DMAs, 2,
+// 8 or 16 tile columns at a time in place of 4 and the barrier elsewhere in the
+// step left the time where it was or made it longer.
 // M and N are at least 256: a last tile that would end past them begins earlier
 // instead, and what it has in common with the one before is written twice, the
 // same bits.  The last steps bring nothing past K: a stage that is not there is

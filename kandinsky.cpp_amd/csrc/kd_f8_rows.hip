@@ -71,8 +71,9 @@ static __device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
     return x > o ? x : o;
 }
 
-// the sum over the 64 lanes, in every lane: of 16 by DPP, then by swaps of
-// rows of 16 and of 32 (a shuffle through LDS takes its latency each step)
+// the sum over each LANES (16, 32 or 64) lanes, in every lane: of 16 by DPP,
+// then by swaps of rows of 16 and of 32 (a shuffle through LDS takes its
+// latency each step)
 template <int CTRL>
 static __device__ __forceinline__ double add_dpp(double x) {
     const uint64_t u = __builtin_bit_cast(uint64_t, x);
@@ -80,16 +81,31 @@ static __device__ __forceinline__ double add_dpp(double x) {
     const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
     return x + __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
-static __device__ __forceinline__ double wave_sum(double x) {
+template <int LANES>
+static __device__ __forceinline__ double lane_sum(double x) {
     x = add_dpp<0xb1>(x);    // lane ^ 1
     x = add_dpp<0x4e>(x);    // lane ^ 2
     x = add_dpp<0x141>(x);   // 7 - lane of each 8
     x = add_dpp<0x140>(x);   // 15 - lane
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
-    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
-    return pair_sum_f64(__builtin_bit_cast(double, (uint64_t)lo[0] | ((uint64_t)hi[0] << 32)) +
-                        __builtin_bit_cast(double, (uint64_t)lo[1] | ((uint64_t)hi[1] << 32)));
+    if constexpr (LANES >= 32) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+        x = __builtin_bit_cast(double, (uint64_t)lo[0] | ((uint64_t)hi[0] << 32)) +
+            __builtin_bit_cast(double, (uint64_t)lo[1] | ((uint64_t)hi[1] << 32));
+    }
+    if constexpr (LANES >= 64) x = pair_sum_f64(x);
+    return x;
+}
+
+// 1 / sqrt(v) of v >= 0 within 2^-50: v_rsq_f64 and two steps of Newton's
+// method, each of which squares its error (a division and a square root in
+// double are three times the instructions).  0 of infinity.
+static __device__ __forceinline__ double rsqrt_f64(double v) {
+    double r = __builtin_amdgcn_rsq(v);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) r = __builtin_fma(r, __builtin_fma(-0.5 * v * r, r, 0.5), r);
+    return __builtin_isinf(v) ? 0.0 : r;
 }
 
 // Eight values of a block (its 16 lanes call together) as codes; the block's
@@ -179,23 +195,28 @@ __global__ __launch_bounds__(256) void quantize_kernel(F8RowsArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// norm_kernel: T threads to a row, C chunks of 8 values each, the whole row
-// in registers between its one reading and its writing.  Bound by HBM for
+// norm_kernel: LANES lanes of a wave to a row of up to 8 LANES values, or
+// (LANES = 0) a workgroup to a row, C chunks of 8 values a thread; the whole
+// row in registers between its one reading and its writing.  Bound by HBM for
 // many rows (63,488 x 4096, BF16 onto an F32 stream, 2.86 GB: 0.52 ms, 5.5
 // TB/s, what a copy reaches), by one row's latency for few (2 x 3584: 2.8 us).
 // A code is a rounding to 4 bits, and a value next to its border goes to the
 // wrong side by an error of the value's last bits: so the squares are summed in
 // double and each value of the norm is rounded once (both under the loads).
 // ---------------------------------------------------------------------------
-template <int XT, int ST, bool RES, int T, int C>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
-    constexpr int kRows = T < 256 ? 256 / T : 1;   // rows at once in a workgroup
-    constexpr int kWaves = T / 64;
-    __shared__ double part[2][kWaves];
-    const int tid = threadIdx.x % T;
+template <int XT, int ST, bool RES, int LANES, int C>
+__global__ __launch_bounds__(LANES ? 256 : 1024) void norm_kernel(F8RowsArgs a) {
+    constexpr int kRows = LANES ? 256 / LANES : 1;   // rows at once in a workgroup
+    __shared__ double part[2][16];
+    const int T = LANES ? LANES : blockDim.x;
+    const int tid = LANES ? threadIdx.x % LANES : threadIdx.x;
     const int lane = threadIdx.x & 63;
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T; row < a.M; row += (int64_t)gridDim.x * kRows) {
+    for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.M; base += (int64_t)gridDim.x * kRows) {
+        // past the end, the last row again (not stored)
+        const int64_t mine = base + (LANES ? threadIdx.x / LANES : 0);
+        const bool live = mine < a.M;
+        const int64_t row = live ? mine : a.M - 1;
         F8Src<XT> x[C];
         F8Src<ST> r[C];
 #pragma unroll
@@ -227,7 +248,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
                 r[c].get(z);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[c][e] += z[e];
-                F8Src<ST>::round_store(a.sum + row * a.s_nb1, col, y[c], in);
+                F8Src<ST>::round_store(a.sum + row * a.s_nb1, col, y[c], in && live);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -235,21 +256,19 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
                 ss += (double)y[c][e] * (double)y[c][e];
             }
         }
-        ss = wave_sum(ss);
-        if constexpr (kWaves > 1) {
+        ss = lane_sum<LANES ? LANES : 64>(ss);
+        if constexpr (LANES == 0) {
             // two buffers in turn: a row's partial sums are read before the
             // next row's barrier, the row after that writes over them behind it
-            if (lane == 0) part[turn][tid >> 6] = ss;
+            if (lane == 0) part[turn][threadIdx.x >> 6] = ss;
             __syncthreads();
-            ss = 0.0;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) ss += part[turn][w];
+            ss = lane_sum<16>((lane & 15) < T >> 6 ? part[turn][lane & 15] : 0.0);
             turn ^= 1;
         }
         // 1 / rms as the sum of two F32; of rows so small or large that these
         // would not be normal numbers, 2^100 goes over to y (exact, but for
         // what is nothing beside the row's largest)
-        double rstd = 1.0 / __builtin_sqrt(ss / (double)a.K + (double)a.eps);
+        double rstd = rsqrt_f64(__builtin_fma(ss, a.inv_k, (double)a.eps));
         if (!(rstd >= 0x1p-100 && rstd <= 0x1p100)) {
             const float up = rstd > 1.0 ? 0x1p100f : 0x1p-100f;
             rstd *= rstd > 1.0 ? 0x1p-100 : 0x1p100;
@@ -278,7 +297,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void norm_kernel(F8RowsArgs a) {
             }
             uint32_t byte;
             const u32x2 q = to_f8(v, byte);
-            if (in) {
+            if (in && live) {
                 *reinterpret_cast<u32x2 *>(a.codes + row * a.c_nb1 + col) = q;
                 if ((tid & 15) == 0) a.scales[row * a.e_nb1 + (col >> 7)] = (char)byte;
             }
@@ -298,25 +317,29 @@ hipError_t launch_f8_quantize(const F8RowsArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int XT, int ST, bool RES, int T, int C>
-static void launch_norm_tc(const F8RowsArgs &a, hipStream_t s) {
-    constexpr int kRows = T < 256 ? 256 / T : 1;
+template <int XT, int ST, bool RES, int LANES, int C>
+static void launch_norm_c(const F8RowsArgs &a, hipStream_t s) {
+    constexpr int kRows = LANES ? 256 / LANES : 1;
     const int64_t want = ((int64_t)a.M + kRows - 1) / kRows;
     const dim3 grid((unsigned)(want < (1 << 20) ? want : 1 << 20));
-    hipLaunchKernelGGL((norm_kernel<XT, ST, RES, T, C>), grid, dim3(T < 256 ? 256 : T), 0, s, a);
+    const int threads = LANES ? 256 : (a.K + 512 * C - 1) / (512 * C) * 64;
+    hipLaunchKernelGGL((norm_kernel<XT, ST, RES, LANES, C>), grid, dim3(threads), 0, s, a);
 }
 
 template <int XT, int ST, bool RES>
 static void launch_norm_t(const F8RowsArgs &a, hipStream_t s) {
     // as few values a thread as a workgroup allows: at any number of rows no
     // slower than a wave to a row, which 2 rows of 3,584 take 5.5 us and 8,192
-    // rows 72 (here 2.8 and 63)
-    if (a.K <= 512) launch_norm_tc<XT, ST, RES, 64, 1>(a, s);
-    else if (a.K <= 2048) launch_norm_tc<XT, ST, RES, 256, 1>(a, s);
-    else if (a.K <= 4096) launch_norm_tc<XT, ST, RES, 512, 1>(a, s);
-    else if (a.K <= 8192) launch_norm_tc<XT, ST, RES, 1024, 1>(a, s);
-    else if (a.K <= 16384) launch_norm_tc<XT, ST, RES, 1024, 2>(a, s);
-    else launch_norm_tc<XT, ST, RES, 1024, 4>(a, s);
+    // rows 72 (here 2.8 and 63).  What a wave does once a row is half of its
+    // instructions, and they bind where lanes are idle: so no more lanes than
+    // have values (63,488 rows of F32: 128 long 7.9 us on 16 lanes, 22.7 on 64;
+    // 528 long 37 on two waves, 80 on four)
+    if (a.K <= 128) launch_norm_c<XT, ST, RES, 16, 1>(a, s);
+    else if (a.K <= 256) launch_norm_c<XT, ST, RES, 32, 1>(a, s);
+    else if (a.K <= 512) launch_norm_c<XT, ST, RES, 64, 1>(a, s);
+    else if (a.K <= 8192) launch_norm_c<XT, ST, RES, 0, 1>(a, s);
+    else if (a.K <= 16384) launch_norm_c<XT, ST, RES, 0, 2>(a, s);
+    else launch_norm_c<XT, ST, RES, 0, 4>(a, s);
 }
 
 hipError_t launch_f8_norm(const F8RowsArgs &a, hipStream_t s) {

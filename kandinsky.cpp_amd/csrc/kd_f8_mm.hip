@@ -97,20 +97,18 @@ static __device__ __forceinline__ void store_rows(const F8MmArgs &a, const lds_t
 // fragments go into registers at once, and its buffer to stage S on: what is
 // on its way is the whole of LDS, whatever the tile.
 //
-// The scales of a run (of 32 stages of it, if it is longer) are brought ahead
-// of its first stage, row by row in words, and read a byte at a time.
+// The scales come row by row in words of four stages, into one of two slots
+// ahead of the first of the four, and are read a byte at a time.
 // In LDS 16-byte chunk c of row r lies at c ^ ((r >> 1) & 7).  Rows past N or
 // M are the last row again (not stored); a chunk past K is its row's first of
 // the stage, X's then zeroed in the registers.
 //
 // With few tokens it is bound by W's way from HBM: 2 x 16384 x 4096 (67 MB)
-// 12.3 us, 5.5 TB/s, what a copy reaches.  300 x 4096 x 4096 takes 12.5 us
+// 12.3 us, 5.5 TB/s, what a copy reaches.  300 x 4096 x 4096 takes 12.0 us
 // (256 tiles of 64 x 80, one on each CU): 4 of it the first loads, the sums and
 // the stores, and 0.2 for each of the 32 stages, whose 18 KB then come into LDS
 // at 23 TB/s over all CUs, out of the L2s.
 // ---------------------------------------------------------------------------
-constexpr int kRingWords = 8;   // words of scales per row at a time
-
 template <int NB, int MB, int S>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void f8_mm_ring(F8MmArgs a) {
@@ -118,12 +116,12 @@ void f8_mm_ring(F8MmArgs a) {
     constexpr int kStage = kRows * 128;
     constexpr int kDma = kRows / 8;                         // of a stage
     constexpr int kWordRows = (kRows + 63) / 64 * 64;       // rows of a word's DMAs
-    constexpr int kScales = kRingWords * kWordRows * 4;
-    constexpr int kWave = S * kStage + kScales;
+    constexpr int kSlot = kWordRows * 4;
+    constexpr int kWave = S * kStage + 2 * kSlot;
     constexpr int PN = NB % 4 == 0 ? 4 : NB % 2 == 0 ? 2 : 1;   // fragments of outputs that are joined at once
     constexpr int kPart = 16 * MB * 16 * PN * 4;
     constexpr int kLds = 4 * (kWave > kPart ? kWave : kPart);
-    static_assert(kLds <= 163840 && (S - 1) * kDma <= 63, "LDS, and the counter of what is on its way");
+    static_assert(kLds <= 163840 && S <= 4 && (S - 1) * kDma <= 63, "LDS, a slot of words that is read before it is written again, and the counter of what is on its way");
     __shared__ __attribute__((aligned(1024))) char lds[kLds];
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -151,11 +149,26 @@ void f8_mm_ring(F8MmArgs a) {
     const int nk = (int)(((uint32_t)a.K + 127) >> 7);
     // this wave's stages
     const int k0 = (int)((int64_t)wave * nk >> 2), k1 = (int)((int64_t)(wave + 1) * nk >> 2);
-    // stage kt into ring buffer buf; past this wave's last, the tile's first
-    // chunk for every lane (not used), so that the counter counts alike
+    // word g of the tile's rows: W's, then X's, then X's last again
+    const char *word_at[kWordRows / 64];
+#pragma unroll
+    for (int h = 0; h < kWordRows / 64; ++h) {
+        const int r = 64 * h + lane, rx = r - 16 * NB;
+        word_at[h] = rx < 0 ? a.ws + (int64_t)(n0 + min(r, w_last)) * a.ws_nb1
+                            : a.xs + (int64_t)(m0 + min(min(rx, 16 * MB - 1), x_last)) * a.xs_nb1;
+    }
+    auto issue_word = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < kWordRows / 64; ++h) dma_word(word_at[h] + 4 * (int64_t)g, words + (g & 1) * kSlot + h * 256);
+    };
+    // stage kt into ring buffer buf, its word before the first of four; past
+    // this wave's last, the tile's first chunk for every lane (not used), so
+    // that the counter counts alike (the words are not counted: a wait is then
+    // for up to as many operations of the next stage too)
     auto issue = [&](int kt, int buf) __attribute__((always_inline)) {
         lds_t *const to = ring + buf * kStage;
         if (kt < k1) {
+            if ((kt & 3) == 0) issue_word(kt >> 2);
             const int64_t kb = (int64_t)kt * 128;
             const int left = a.K - kt * 128;
             const uint32_t b0 = 16 * c0 < left ? 16 * c0 : 0, b1 = 16 * c1 < left ? 16 * c1 : 0;
@@ -166,17 +179,6 @@ void f8_mm_ring(F8MmArgs a) {
             for (int j = 0; j < kDma; ++j) dma_16b(j < 2 * NB ? wt : xt, 0, to + j * 1024);
         }
     };
-    // words first .. +count-1 of the tile's rows, [word][row]
-    auto issue_words = [&](int first, int count) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < kWordRows / 64; ++h) {
-            // a lane's row: W's, then X's, then X's last again
-            const int r = 64 * h + lane, rx = r - 16 * NB;
-            const bool w = rx < 0;
-            const char *const p = w ? a.ws + (int64_t)(n0 + min(r, w_last)) * a.ws_nb1 : a.xs + (int64_t)(m0 + min(min(rx, 16 * MB - 1), x_last)) * a.xs_nb1;
-            for (int c = 0; c < count; ++c) dma_word(p + 4 * (int64_t)(first + c), words + c * kWordRows * 4 + h * 256);
-        }
-    };
 
     f32x4 acc[NB][MB];
 #pragma unroll
@@ -185,18 +187,17 @@ void f8_mm_ring(F8MmArgs a) {
         for (int j = 0; j < MB; ++j) acc[i][j] = (f32x4){};
     typedef const __attribute__((address_space(3))) u32x4 lds_u4;
     const uint32_t f_rd = (uint32_t)(l16 * 128 + ((q4 ^ ((l16 >> 1) & 7)) << 4));
-    for (int ka = k0; ka < k1;) {   // runs of up to kRingWords words
-        const int first = ka >> 2, kb = min(k1, 4 * (first + kRingWords));
-        issue_words(first, ((kb + 3) >> 2) - first);
+    if (k0 < k1) {
+        if (k0 & 3) issue_word(k0 >> 2);
 #pragma unroll
-        for (int s = 0; s < S; ++s) issue(ka + s, s);
+        for (int s = 0; s < S; ++s) issue(k0 + s, s);
         int buf = 0;
-        for (int kt = ka; kt < kb; ++kt) {
+        for (int kt = k0; kt < k1; ++kt) {
             asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1) * kDma) : "memory");
             const lds_t *const from = ring + buf * kStage;
             u32x4 fw[NB][2], fx[MB][2];
             uint32_t sw[NB], sx[MB];
-            const lds_t *const sp = words + ((kt >> 2) - first) * kWordRows * 4 + (kt & 3) + l16 * 4;
+            const lds_t *const sp = words + ((kt >> 2) & 1) * kSlot + (kt & 3) + l16 * 4;
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 sw[i] = *reinterpret_cast<const __attribute__((address_space(3))) uint8_t *>(sp + 64 * i);
@@ -227,9 +228,8 @@ void f8_mm_ring(F8MmArgs a) {
                 for (int j = 0; j < MB; ++j)
                     acc[i][j] = mfma_f8(join(fw[i][0], fw[i][1]), join(fx[j][0], fx[j][1]), acc[i][j], sw[i], sx[j]);
         }
-        // what is still on its way is the next run's (or nobody's)
+        // what is still on its way is nobody's
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        ka = kb;
     }
 
     // ---- the four partial sums, 16 PN outputs of every token at a time: row

@@ -272,6 +272,8 @@ int kd_f8_mm_run(const kd_f8_mm_desc *desc, void *stream) {
     a.tiles_m = (int32_t)tiles_m;
     a.n_blocks = (int32_t)(tiles_n * tiles_m);
     a.cols = 4;
+    // (code rows that do not all start on 128-byte lines, where that pays)
+    a.lines = K >= 1024 && (!aligned(desc->w.codes.data, 128) || !aligned(desc->x.codes.data, 128) || !aligned((uint64_t)(a.w_nb1 | a.x_nb1), 128));
     return launched(kdfa::launch_f8_mm(a, tile, static_cast<hipStream_t>(stream)));
 }
 

@@ -282,10 +282,17 @@ void f8_mm_ring(F8MmArgs a) {
 // 1,280 x 4096 x 4096 takes 23.5 us (256 tiles of 128 x 160, one on each CU):
 // 0.46 us a stage for the CU's 36 KB into LDS, 20 TB/s over all of them out of
 // the L2s, where the products would take 0.31 at the rate they sustain.  997 x
-// 1540 x 3600: 17.8 us (208 tiles of 128 x 64), 13.1 with the rows padded to
-// whole lines.
+// 1540 x 3600: 14 us (208 tiles of 128 x 64).
+//
+// LINES, for code rows that do not all start on 128-byte lines: a stage brings
+// a line of each row in place of 128 k, the first and last clamped to the row,
+// and a block's chunks are read out of two stages.  128 k of such a row cross
+// two lines, each of which came twice: 997 x 1540 x 3600 (rows packed) 17.8 us,
+// so 14.0; 1,280 x 4096 x 3600 26.2 and 22.3.  The one more stage that it waits
+// for costs 0.2-0.3 us below eight blocks (1500 x 1500 x 400 6.8 and 7.1): from
+// K = 1024 on.
 // ---------------------------------------------------------------------------
-template <int NB, int MB, int S>
+template <int NB, int MB, int S, bool LINES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void f8_mm_grid(F8MmArgs a) {
     constexpr int kRows = 32 * (NB + MB);
@@ -296,7 +303,7 @@ void f8_mm_grid(F8MmArgs a) {
     constexpr int kWaveOut = 16 * MB * 32 * NB;       // a wave's part of dst
     constexpr int kUse = S * kStage + 2 * kSlot;
     constexpr int kLds = kUse > 4 * kWaveOut ? kUse : 4 * kWaveOut;
-    static_assert(kLds <= 163840 && S >= 2 && S <= 8, "LDS, and a slot of words that is read before it is written again");
+    static_assert(kLds <= 163840 && S >= 2 + LINES && S <= 8, "LDS, and a slot of words that is read before it is written again");
     __shared__ __attribute__((aligned(1024))) char lds[kLds];
     lds_t *const sbase = LDS_PTR(char, lds);
     lds_t *const words = sbase + S * kStage;
@@ -320,10 +327,20 @@ void f8_mm_grid(F8MmArgs a) {
     // chunk that lies at l % 8 of row l / 8
     uint32_t off[kDma];
     const int dc = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+    // LINES: row r begins (at + r * step) % 8 chunks of 16 bytes into a line,
+    // rows r + 8, r + 16 .. too.  A row's chunk c of a block then lies at the
+    // same place of the buffer as without (no other banks), of this stage's
+    // line or of the next one; rel is the byte of line 0, from the row's
+    // first, that this lane brings.
+    const int w_step = (int)(a.w_nb1 >> 4) & 7, x_step = (int)(a.x_nb1 >> 4) & 7;
+    const int w_at = (int)((uintptr_t)wt >> 4) & 7, x_at = (int)((uintptr_t)xt >> 4) & 7;
+    const int w_sh = (w_at + (lane >> 3) * w_step) & 7, x_sh = (x_at + (lane >> 3) * x_step) & 7;
+    const int w_rel = 16 * (((dc + w_sh) & 7) - w_sh), x_rel = 16 * (((dc + x_sh) & 7) - x_sh);
 #pragma unroll
     for (int j = 0; j < kDma; ++j) {
         const int r = 8 * (wave + 4 * j) + (lane >> 3);
         off[j] = j < NB ? (uint32_t)min(r, w_last) * (uint32_t)a.w_nb1 : (uint32_t)min(r - 32 * NB, x_last) * (uint32_t)a.x_nb1;
+        if constexpr (LINES) off[j] += 128 + (j < NB ? w_rel : x_rel);
     }
     // DMA h of a word: rows 256 h + 64 wave + lane (W's, X's, X's last again)
     const char *word_at[kWordDma];
@@ -341,6 +358,19 @@ void f8_mm_grid(F8MmArgs a) {
 #pragma unroll
                 for (int h = 0; h < kWordDma; ++h) dma_word(word_at[h] + 4 * (int64_t)g, words + ((kt >> 2) & 1) * kSlot + h * 1024 + wave * 256);
             }
+        }
+        if constexpr (LINES) {
+            // (from 128 bytes before the tile, so that no offset is negative)
+            const char *at = (j < NB ? wt : xt) + ((int64_t)kt - 1) * 128;
+            uint32_t o = off[j];
+            if constexpr (decltype(end_c)::value) {
+                // outside of the row, its first or last chunk
+                const int rel = kt * 128 + (j < NB ? w_rel : x_rel);
+                o = kt > nk ? 128 : o + (uint32_t)(min(max(rel, 0), a.K - 16) - rel);
+                at = kt > nk ? (j < NB ? wt : xt) - 128 : at;
+            }
+            dma_16b(at, o, sbase + buf * kStage + (wave + 4 * j) * 1024);
+            return;
         }
         const char *at = (j < NB ? wt : xt) + (int64_t)kt * 128;
         uint32_t o = off[j] + (uint32_t)(dc << 4);
@@ -362,9 +392,29 @@ void f8_mm_grid(F8MmArgs a) {
     const uint32_t w_rd = f_rd + 16 * NB * wn * 128, x_rd = f_rd + (32 * NB + 16 * MB * wm) * 128;
     u32x4 fw[2][NB][2], fx[2][MB][2];
     uint32_t sw[NB], sx[MB], nw[NB], nx[MB];
+    // LINES: all bits where chunk q4 or q4 + 4 of a block is in the next line
+    uint32_t w_next[2], x_next[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w_next[h] = 0u - (uint32_t)((q4 + 4 * h + ((w_at + l16 * w_step) & 7)) >> 3);
+        x_next[h] = 0u - (uint32_t)((q4 + 4 * h + ((x_at + l16 * x_step) & 7)) >> 3);
+    }
     auto read = [&](int buf, auto set_c) __attribute__((always_inline)) {
         constexpr int set = decltype(set_c)::value;
         const lds_t *const from = sbase + buf * kStage;
+        if constexpr (LINES) {
+            const uint32_t here = buf * kStage, on = buf == S - 1 ? 0u - (S - 1) * kStage : kStage;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const lds_t *const wf = sbase + ((w_rd ^ (h << 6)) + here + (w_next[h] & on));
+                const lds_t *const xf = sbase + ((x_rd ^ (h << 6)) + here + (x_next[h] & on));
+#pragma unroll
+                for (int i = 0; i < NB; ++i) fw[set][i][h] = *reinterpret_cast<lds_u4 *>(wf + i * 2048);
+#pragma unroll
+                for (int j = 0; j < MB; ++j) fx[set][j][h] = *reinterpret_cast<lds_u4 *>(xf + j * 2048);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -394,7 +444,7 @@ void f8_mm_grid(F8MmArgs a) {
         constexpr int Q = decltype(sel_c)::value, P = Q & 1;
         const int here = buf;
         buf = buf == S - 1 ? 0 : buf + 1;
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(later(Q, 2)) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(later(Q, 2 + LINES)) : "memory");
         __syncthreads();
         read(buf, IC<1 - P>());
         if constexpr (Q == 3) read_words((kt >> 2) + 1);
@@ -433,7 +483,7 @@ void f8_mm_grid(F8MmArgs a) {
 #pragma unroll
         for (int j = 0; j < kDma; ++j) dma_j(s, s, j, BC<s % 4 == 0>(), BC<true>());
     });
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(later(0, 1)) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(later(0, 1 + LINES)) : "memory");
     __syncthreads();
     read(0, IC<0>());
     read_words(0);
@@ -777,9 +827,13 @@ static void launch_ring(const F8MmArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((f8_mm_ring<NB, MB, S>), dim3(a.n_blocks), dim3(256), 0, s, a);
 }
 
-template <int NB, int MB, int S>
+template <int NB, int MB, int S, int LS>
 static void launch_grid(const F8MmArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((f8_mm_grid<NB, MB, S>), dim3(a.n_blocks), dim3(256), 0, s, a);
+    if (a.lines) {
+        hipLaunchKernelGGL((f8_mm_grid<NB, MB, LS, true>), dim3(a.n_blocks), dim3(256), 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((f8_mm_grid<NB, MB, S, false>), dim3(a.n_blocks), dim3(256), 0, s, a);
 }
 
 hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t s) {
@@ -789,10 +843,10 @@ hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t s) {
     case 401: launch_ring<4, 1, 3>(a, s); break;
     case 402: launch_ring<4, 2, 3>(a, s); break;
     case 405: launch_ring<4, 5, 1>(a, s); break;
-    case 10804: launch_grid<4, 2, 5>(a, s); break;
-    case 10806: launch_grid<4, 3, 5>(a, s); break;
-    case 10810: launch_grid<4, 5, 4>(a, s); break;
-    case 10816: launch_grid<4, 8, 3>(a, s); break;
+    case 10804: launch_grid<4, 2, 5, 5>(a, s); break;
+    case 10806: launch_grid<4, 3, 5, 5>(a, s); break;
+    case 10810: launch_grid<4, 5, 4, 4>(a, s); break;
+    case 10816: launch_grid<4, 8, 3, 3>(a, s); break;
     case 11616: hipLaunchKernelGGL(f8_mm_tile, dim3(a.n_blocks), dim3(256), 0, s, a); break;
     default: return hipErrorInvalidValue;
     }

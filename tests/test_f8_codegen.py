@@ -22,7 +22,7 @@ def _named(part):
 
 
 def test_every_kernel_is_here():
-    assert len(_named("f8_mm_tile")) == 1 and len(_named("f8_mm_ring")) == 5 and len(_named("f8_mm_grid")) == 4
+    assert len(_named("f8_mm_tile")) == 1 and len(_named("f8_mm_ring")) == 5 and len(_named("f8_mm_grid")) == 8
 
 
 @pytest.mark.parametrize("source", [SOURCE, "kd_f8_rows.hip"])
@@ -135,11 +135,12 @@ def _runs(kinds):
     yield run
 
 
-@pytest.mark.parametrize("nb,mb,stages", [(4, 2, 5), (4, 3, 5), (4, 5, 4), (4, 8, 3)])
-def test_grid_steps_count_their_dmas(nb, mb, stages):
-    """Four steps: a wait that leaves what was sent behind the next stage, the
-    stages' DMAs and, once, a word's."""
-    name = [n for n in _named("f8_mm_grid") if f"ILi{nb}ELi{mb}ELi{stages}E" in n]
+@pytest.mark.parametrize("nb,mb,stages,lines", [(4, 2, 5, 0), (4, 3, 5, 0), (4, 5, 4, 0), (4, 8, 3, 0), (4, 2, 5, 1), (4, 3, 5, 1), (4, 5, 4, 1), (4, 8, 3, 1)])
+def test_grid_steps_count_their_dmas(nb, mb, stages, lines):
+    """Four steps: a wait that leaves what was sent behind the next stage (the
+    next two, where a block's chunks lie in two lines), the stages' DMAs and,
+    once, a word's."""
+    name = [n for n in _named("f8_mm_grid") if f"ILi{nb}ELi{mb}ELi{stages}ELb{lines}E" in n]
     assert len(name) == 1
     body = _steady(kernels(SOURCE)[name[0]], 4 * nb * mb)
     per, word = nb + mb, (32 * (nb + mb) + 255) // 256
@@ -147,7 +148,7 @@ def test_grid_steps_count_their_dmas(nb, mb, stages):
     assert sum(b.startswith("global_load_lds_dword ") for b in body) == word
     assert sum(b == "s_barrier" for b in body) == 4
     left = [int(re.match(r"s_waitcnt vmcnt\((\d+)\) lgkmcnt\(0\)", b).group(1)) for b in body if re.match(r"s_waitcnt vmcnt\(\d+\) lgkmcnt\(0\)", b)]
-    want = [sum(per + (word if (q + t) % 4 == 0 else 0) for t in range(2, stages)) for q in range(4)]
+    want = [sum(per + (word if (q + t) % 4 == 0 else 0) for t in range(2 + lines, stages)) for q in range(4)]
     assert left == want
 
 

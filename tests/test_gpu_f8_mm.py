@@ -151,6 +151,29 @@ def test_nan_rows_stay_in_their_rows():
     assert torch.equal(got[keep], round_bf16(want)[keep])
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 64, 2064), (40, 4096, 1040), (77, 2732, 3120), (96, 3000, 4096), (300, 1500, 1552), (559, 444, 2048),
+                                   (1292, 1500, 2096), (1999, 1024, 144), (700, 1028, 16), (1406, 4208, 1280), (2300, 3300, 1664)])
+@pytest.mark.parametrize("lead,gap", [(16, 0), (112, 16), (0, 144), (64, 64), (48, 368)])
+def test_rows_that_start_anywhere_in_a_line(M, N, K, lead, gap):
+    """Codes `lead` bytes behind the start of a line, `gap` bytes between the
+    rows, NaN in all that is not theirs."""
+    _need_gpu()
+    announce(f"mm {M} x {N} x {K} at {lead}, {gap} apart")
+    x, w, b, want = _exact(M, N, K, True)
+
+    def elsewhere(r, lead, gap):
+        rows = r.codes.shape[0]
+        store = torch.full((lead + rows * (K + gap) + 256,), 0x7F, dtype=torch.uint8, device=DEV)
+        codes = store[lead:lead + rows * (K + gap)].view(rows, K + gap)[:, :K]
+        codes.copy_(r.codes.view(torch.uint8))
+        return kd_f8.Rows(codes.view(torch.float8_e4m3fn), r.scales)
+
+    for xs, ws in (((lead, gap), (0, (-K) % 128)), ((0, (-K) % 128), (lead, gap)), ((lead, gap), (gap, lead))):
+        got = kd_f8.linear(elsewhere(x, *xs), elsewhere(w, *ws), b)
+        torch.cuda.synchronize()
+        assert torch.equal(got.cpu(), want), (xs, ws)
+
+
 def test_rows_of_three_dimensions_and_strided_operands():
     _need_gpu()
     announce("mm 3-D strided")

@@ -38,7 +38,7 @@ struct F8MmArgs {
     int64_t w_nb1, x_nb1, ws_nb1, xs_nb1, d_nb1;
     int32_t M, N, K;
     int32_t tiles_m, tiles_n, n_blocks, cols;
-    int32_t lines;          // f8_mm_grid's LINES
+    int32_t lines;          // f8_mm_ring's and f8_mm_grid's LINES
 };
 
 constexpr int64_t kF8MmMaxBlocks = 1 << 23;   // workgroups of 256 threads in one launch, with room to spare

@@ -108,8 +108,15 @@ static __device__ __forceinline__ void store_rows(const F8MmArgs &a, const lds_t
 // (256 tiles of 64 x 80, one on each CU): 4 of it the first loads, the sums and
 // the stores, and 0.2 for each of the 32 stages, whose 18 KB then come into LDS
 // at 23 TB/s over all CUs, out of the L2s.
+//
+// LINES, for code rows that do not all start on 128-byte lines: a stage brings
+// a line of each row in place of 128 k, what is not the row's its first or last
+// chunk again, and a block's chunks are read out of two stages: 128 k of such a
+// row cross two lines, each of which came twice.  From K = 1024 on (packed rows,
+// 300 x 4096 x 4112 15.3 us, so 13.0; x 1040 7.6 and 7.4; x 528 5.9 and 6.4; 17 x
+// 260 x 4112, where it only waits longer, 4.7 and 5.5).
 // ---------------------------------------------------------------------------
-template <int NB, int MB, int S>
+template <int NB, int MB, int S, bool LINES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
 void f8_mm_ring(F8MmArgs a) {
     constexpr int kRows = 16 * (NB + MB);
@@ -121,7 +128,7 @@ void f8_mm_ring(F8MmArgs a) {
     constexpr int PN = NB % 4 == 0 ? 4 : NB % 2 == 0 ? 2 : 1;   // fragments of outputs that are joined at once
     constexpr int kPart = 16 * MB * 16 * PN * 4;
     constexpr int kLds = 4 * (kWave > kPart ? kWave : kPart);
-    static_assert(kLds <= 163840 && S <= 4 && (S - 1) * kDma <= 63, "LDS, a slot of words that is read before it is written again, and the counter of what is on its way");
+    static_assert(kLds <= 163840 && S >= 1 + LINES && S <= 4 && (S - 1) * kDma <= 63, "LDS, a slot of words that is read before it is written again, and the counter of what is on its way");
     __shared__ __attribute__((aligned(1024))) char lds[kLds];
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -146,6 +153,10 @@ void f8_mm_ring(F8MmArgs a) {
         off[j] = j < 2 * NB ? (uint32_t)min(r, w_last) * (uint32_t)a.w_nb1 : (uint32_t)min(r - 16 * NB, x_last) * (uint32_t)a.x_nb1;
     }
     const int c0 = (lane & 7) ^ (lane >> 4), c1 = c0 ^ 4;   // chunks of even and odd j
+    // LINES: where a row begins in its line, in chunks (row r as r + 8)
+    const int w_step = (int)(a.w_nb1 >> 4) & 7, x_step = (int)(a.x_nb1 >> 4) & 7;
+    const int w_at = (int)((uintptr_t)wt >> 4) & 7, x_at = (int)((uintptr_t)xt >> 4) & 7;
+    const int w_sh = (w_at + (lane >> 3) * w_step) & 7, x_sh = (x_at + (lane >> 3) * x_step) & 7;
     const int nk = (int)(((uint32_t)a.K + 127) >> 7);
     // this wave's stages
     const int k0 = (int)((int64_t)wave * nk >> 2), k1 = (int)((int64_t)(wave + 1) * nk >> 2);
@@ -167,8 +178,21 @@ void f8_mm_ring(F8MmArgs a) {
     // for up to as many operations of the next stage too)
     auto issue = [&](int kt, int buf) __attribute__((always_inline)) {
         lds_t *const to = ring + buf * kStage;
-        if (kt < k1) {
-            if ((kt & 3) == 0) issue_word(kt >> 2);
+        if (kt < k1 + LINES) {
+            if ((kt & 3) == 0 && kt < k1) issue_word(kt >> 2);
+            if constexpr (LINES) {
+                // (from 128 bytes before the tile, so that no offset is
+                // negative); outside of the row, its first or last chunk
+                const int line = kt * 128;
+                auto at = [&](int c, int sh) __attribute__((always_inline)) {
+                    return (uint32_t)(min(max(line + 16 * (((c + sh) & 7) - sh), 0), a.K - 16) - line + 128);
+                };
+                const uint32_t w0 = at(c0, w_sh), w1 = at(c1, w_sh), x0 = at(c0, x_sh), x1 = at(c1, x_sh);
+#pragma unroll
+                for (int j = 0; j < kDma; ++j)
+                    dma_16b((j < 2 * NB ? wt : xt) + (int64_t)line - 128, off[j] + (j < 2 * NB ? (j & 1 ? w1 : w0) : (j & 1 ? x1 : x0)), to + j * 1024);
+                return;
+            }
             const int64_t kb = (int64_t)kt * 128;
             const int left = a.K - kt * 128;
             const uint32_t b0 = 16 * c0 < left ? 16 * c0 : 0, b1 = 16 * c1 < left ? 16 * c1 : 0;
@@ -187,28 +211,38 @@ void f8_mm_ring(F8MmArgs a) {
         for (int j = 0; j < MB; ++j) acc[i][j] = (f32x4){};
     typedef const __attribute__((address_space(3))) u32x4 lds_u4;
     const uint32_t f_rd = (uint32_t)(l16 * 128 + ((q4 ^ ((l16 >> 1) & 7)) << 4));
+    // LINES: all bits where chunk q4 or q4 + 4 of a block is in the next line
+    uint32_t w_next[2], x_next[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w_next[h] = 0u - (uint32_t)((q4 + 4 * h + ((w_at + l16 * w_step) & 7)) >> 3);
+        x_next[h] = 0u - (uint32_t)((q4 + 4 * h + ((x_at + l16 * x_step) & 7)) >> 3);
+    }
     if (k0 < k1) {
         if (k0 & 3) issue_word(k0 >> 2);
 #pragma unroll
         for (int s = 0; s < S; ++s) issue(k0 + s, s);
         int buf = 0;
         for (int kt = k0; kt < k1; ++kt) {
-            asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1) * kDma) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1 - LINES) * kDma) : "memory");
             const lds_t *const from = ring + buf * kStage;
+            const uint32_t on = LINES ? (buf == S - 1 ? 0u - (S - 1) * kStage : kStage) : 0u;
+            const lds_t *const w_from[2] = {from + f_rd + (w_next[0] & on), from + (f_rd ^ 64) + (w_next[1] & on)};
+            const lds_t *const x_from[2] = {from + f_rd + (x_next[0] & on), from + (f_rd ^ 64) + (x_next[1] & on)};
             u32x4 fw[NB][2], fx[MB][2];
             uint32_t sw[NB], sx[MB];
             const lds_t *const sp = words + ((kt >> 2) & 1) * kSlot + (kt & 3) + l16 * 4;
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 sw[i] = *reinterpret_cast<const __attribute__((address_space(3))) uint8_t *>(sp + 64 * i);
-                fw[i][0] = *reinterpret_cast<lds_u4 *>(from + f_rd + i * 2048);
-                fw[i][1] = *reinterpret_cast<lds_u4 *>(from + (f_rd ^ 64) + i * 2048);
+                fw[i][0] = *reinterpret_cast<lds_u4 *>(w_from[0] + i * 2048);
+                fw[i][1] = *reinterpret_cast<lds_u4 *>(w_from[1] + i * 2048);
             }
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
                 sx[j] = *reinterpret_cast<const __attribute__((address_space(3))) uint8_t *>(sp + 64 * (NB + j));
-                fx[j][0] = *reinterpret_cast<lds_u4 *>(from + f_rd + (NB + j) * 2048);
-                fx[j][1] = *reinterpret_cast<lds_u4 *>(from + (f_rd ^ 64) + (NB + j) * 2048);
+                fx[j][0] = *reinterpret_cast<lds_u4 *>(x_from[0] + (NB + j) * 2048);
+                fx[j][1] = *reinterpret_cast<lds_u4 *>(x_from[1] + (NB + j) * 2048);
             }
             // the buffer is free when its reads have returned
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -284,13 +318,8 @@ void f8_mm_ring(F8MmArgs a) {
 // the L2s, where the products would take 0.31 at the rate they sustain.  997 x
 // 1540 x 3600: 14 us (208 tiles of 128 x 64).
 //
-// LINES, for code rows that do not all start on 128-byte lines: a stage brings
-// a line of each row in place of 128 k, the first and last clamped to the row,
-// and a block's chunks are read out of two stages.  128 k of such a row cross
-// two lines, each of which came twice: 997 x 1540 x 3600 (rows packed) 17.8 us,
-// so 14.0; 1,280 x 4096 x 3600 26.2 and 22.3.  The one more stage that it waits
-// for costs 0.2-0.3 us below eight blocks (1500 x 1500 x 400 6.8 and 7.1): from
-// K = 1024 on.
+// LINES as f8_mm_ring's: 997 x 1540 x 3600 (rows packed) 17.8 us without, 14.0
+// with; 1,280 x 4096 x 3600 26.2 and 22.3; 1500 x 1500 x 400 6.8 and 7.1.
 // ---------------------------------------------------------------------------
 template <int NB, int MB, int S, bool LINES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1)))
@@ -822,9 +851,13 @@ void f8_mm_tile(F8MmArgs a) {
     store_rows<128, 16>(a, so, [](int r) { return r & 15; }, m0 + 128 * wm, n0 + 128 * wn, lane);
 }
 
-template <int NB, int MB, int S>
+template <int NB, int MB, int S, int LS>
 static void launch_ring(const F8MmArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((f8_mm_ring<NB, MB, S>), dim3(a.n_blocks), dim3(256), 0, s, a);
+    if (a.lines) {
+        hipLaunchKernelGGL((f8_mm_ring<NB, MB, LS, true>), dim3(a.n_blocks), dim3(256), 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((f8_mm_ring<NB, MB, S, false>), dim3(a.n_blocks), dim3(256), 0, s, a);
 }
 
 template <int NB, int MB, int S, int LS>
@@ -838,11 +871,11 @@ static void launch_grid(const F8MmArgs &a, hipStream_t s) {
 
 hipError_t launch_f8_mm(const F8MmArgs &a, int tile, hipStream_t s) {
     switch (tile) {
-    case 101: launch_ring<1, 1, 4>(a, s); break;
-    case 202: launch_ring<2, 2, 4>(a, s); break;
-    case 401: launch_ring<4, 1, 3>(a, s); break;
-    case 402: launch_ring<4, 2, 3>(a, s); break;
-    case 405: launch_ring<4, 5, 1>(a, s); break;
+    case 101: launch_ring<1, 1, 4, 4>(a, s); break;
+    case 202: launch_ring<2, 2, 4, 4>(a, s); break;
+    case 401: launch_ring<4, 1, 3, 3>(a, s); break;
+    case 402: launch_ring<4, 2, 3, 3>(a, s); break;
+    case 405: launch_ring<4, 5, 1, 2>(a, s); break;
     case 10804: launch_grid<4, 2, 5, 5>(a, s); break;
     case 10806: launch_grid<4, 3, 5, 5>(a, s); break;
     case 10810: launch_grid<4, 5, 4, 4>(a, s); break;

@@ -109,11 +109,18 @@ def empty_rows(rows, K: int, device) -> Rows:
 
 
 _RUN = {}
+_current_device = _current_stream = None   # () -> index, index -> handle
 
 
 def _lib():
+    global _current_device, _current_stream
     lib = kd_fa.lib()
     if not _RUN:
+        torch = kd_fa._torch()
+        # a small call is the host's time: torch.cuda's functions of these are
+        # 2.5 of its 7 us (current_stream makes a Stream object)
+        _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda i: torch.cuda.current_stream(i).cuda_stream)
         P, ci, cv = ctypes.POINTER, ctypes.c_int, ctypes.c_void_p
         for desc, sup, run_ in ((KdF8QuantizeDesc, lib.kd_f8_quantize_supports, lib.kd_f8_quantize),
                                 (KdF8NormDesc, lib.kd_f8_norm_supports, lib.kd_f8_norm_run),
@@ -148,12 +155,14 @@ def _checked(d, what, *tensors):
     """d, if the library can execute it; it keeps the tensors alive."""
     d._keep = tuple(t for t in tensors if t is not None)
     d._device = d._keep[0].device
+    d._index = d._device.index if d._device.type == "cuda" else None
     d._ref = ctypes.byref(d)
     if any(t.device != d._device for t in d._keep):
         raise ValueError(f"{what}: the tensors are on different devices")
     _lib()
+    supports, d._enqueue = _RUN[type(d)]
     reason = ctypes.c_int(0)
-    if not _RUN[type(d)][0](ctypes.byref(d), ctypes.byref(reason)):
+    if not supports(d._ref, ctypes.byref(reason)):
         raise kd_fa.KdFaError(reason.value, what)
     return d
 
@@ -185,24 +194,15 @@ def linear_desc(x: Rows, w: Rows, dst, bias=None) -> KdF8MmDesc:
 def run(desc, stream=None) -> None:
     """Enqueue a descriptor's operator on `stream` (default: the current
     stream of its tensors' device)."""
-    torch = kd_fa._torch()
-    dev = desc._device
-    if dev.type != "cuda":
-        raise ValueError(f"the tensors are on {dev}, not on a GPU")
-    if torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev):
+    on = desc._index
+    if on is None:
+        raise ValueError(f"the tensors are on {desc._device}, not on a GPU")
+    if _current_device() != on:
+        with kd_fa._torch().cuda.device(on):
             return run(desc, stream)
-    st = _RUN[type(desc)][1](desc._ref, _current_stream(dev) if stream is None else stream.cuda_stream)
+    st = desc._enqueue(desc._ref, _current_stream(on) if stream is None else stream.cuda_stream)
     if st != kd_fa.OK:
         raise kd_fa.KdFaError(st, type(desc).__name__)
-
-
-def _current_stream(dev) -> int:
-    """The handle of the device's current stream (torch.cuda.current_stream
-    makes a Stream object for it: 1.9 of a small call's 7 us)."""
-    torch = kd_fa._torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(dev.index) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def _made_on(stream):

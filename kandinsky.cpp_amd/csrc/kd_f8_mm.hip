@@ -583,8 +583,8 @@ void f8_mm_grid(F8MmArgs a) {
 // A row's scales come as words of four stages, loaded by the lanes that hold
 // the row, a step ahead of their first use.
 //
-// 63,488 x 4096 x 4096 takes 0.86-0.87 ms (2.45 PFLOP/s), 15,872 x 4096 x 16384
-// 0.74 (2.88); the products alone (no loads, no LDS reads) would take 0.50 of
+// 63,488 x 4096 x 4096 takes 0.85-0.88 ms (2.4-2.5 PFLOP/s), 15,872 x 4096 x 16384
+// 0.72-0.75 (2.9); the products alone (no loads, no LDS reads) would take 0.50 of
 // the former, the DMAs alone 0.53-0.62.  Both together draw the chip down to
 // 2.0-2.1 GHz, and the two run at once but for what the barrier holds up.
 // Tiles kept up by persistent workgroups (the next tile's first stages under
